@@ -246,6 +246,120 @@ int mb_linear_split_dev(mb_ctx* ctx, int M, int N, int K, const float* A, int64_
 int mb_linear_noalloc_dev(mb_ctx* ctx, int M, int N, int K, const float* A, int64_t lda,
                           const float* W, const float* bias, float* C, int64_t ldc, int epi);
 
+/* ------------------------------------------ several hypotheses per voice
+ * Drafted trees over the rings, and beams whose rings follow the choice.  The
+ * reference decodes one hypothesis per voice (runtime.ts:539-561), so these
+ * have no counterpart there; they stand on its ring rules (above).  Rows are
+ * the fused q | k | v rows of the other ring calls. */
+
+/* Device pointers of the context's rings: K and V are
+ * [n_layers][max_seqs][12][capacity][64] in kv_dtype, slot_pos is
+ * [n_layers][max_seqs][capacity].  Any output may be NULL.  They stay valid,
+ * and at their place, until mb_destroy; work on them is ordered by the
+ * caller's streams. */
+int mb_ring_view(mb_ctx* ctx, void** k, void** v, int32_t** slot_pos);
+
+/* Attention of drafted trees: node i < n_nodes[b] of sequence b has its fused
+ * row in qkv [B][rows_max][2304] and its parent in parent[b][i]: an earlier
+ * node (< i), or -1 for a node that follows the cached rows directly.  It
+ * stands at position pos0[b] + (number of its ancestors) and attends
+ *   - the slots of `layer` whose stored position p satisfies p < pos0[b] and
+ *     lies in its window (0 <= its position - p < capacity): rows of an
+ *     earlier draft at pos0[b] and later are not seen;
+ *   - its ancestors' rows and its own, K roped at their positions, K and V
+ *     rounded as the ring would store them.
+ * out [B][rows_max][768] receives each node's attention output: what appending
+ * its ancestors and it one by one (mb_append_attend) would end with, to
+ * rounding.  Rows i >= n_nodes[b] of out are left as they are.  The rings are
+ * not changed.  rows_max is 1 .. 64; n_nodes[b] may be 0.
+ * Sums are fp32 over fp32 products (of the stored bf16 values in bf16 rings). */
+int mb_tree_attention(mb_ctx* ctx, int layer, int B, int rows_max, const float* qkv,
+                      const int32_t* parent, const int32_t* pos0, const int32_t* n_nodes, float* out);
+
+/* Bytes of the workspace that mb_tree_attention_dev takes for B sequences of
+ * rows_max nodes at positions up to max_pos (0: none; a NULL workspace is
+ * right then). */
+int mb_tree_attention_work(mb_ctx* ctx, int B, int rows_max, int32_t max_pos, int64_t* bytes);
+
+/* Device-pointer form (enqueue only).  max_pos bounds every node's position
+ * (a larger bound than needed is right too): it sizes the split of the windows.
+ * n_nodes may be NULL (rows_max each).  qkv_stride and out_stride are in
+ * elements between rows; every row starts at a multiple of 16 bytes.  A parent
+ * that is not an earlier node counts as -1; a sequence whose positions do not
+ * fit int32 (pos0[b] < 0 or > 2^31 - 65) is left out.  `work` holds
+ * mb_tree_attention_work bytes, 16-byte aligned, of any content; calls that may
+ * overlap (on two streams, or two captured graphs' replays) need one each. */
+int mb_tree_attention_dev(mb_ctx* ctx, int layer, int B, int rows_max, const void* qkv,
+                          int qkv_dtype, int64_t qkv_stride, const int32_t* parent,
+                          const int32_t* pos0, const int32_t* n_nodes, int32_t max_pos, float* out,
+                          int64_t out_stride, void* work, int64_t work_bytes);
+
+/* Commit the accepted path of each tree, in n_layers layers from layer0 on:
+ * for i < n_path[b], node path[b][i] of layer l's rows qkv
+ * [n_layers][B][rows_max][2304] is written at position pos0[b] + i, K roped,
+ * as mb_ring_write_rows writes it (the last capacity rows of a longer path).
+ * path is [B][path_max], any nodes in any order; n_path[b] is 0 .. path_max. */
+int mb_tree_commit(mb_ctx* ctx, int layer0, int n_layers, int B, int rows_max, const float* qkv,
+                   const int32_t* pos0, int path_max, const int32_t* path, const int32_t* n_path);
+/* Device-pointer form (enqueue only): one launch for all layers, layer_stride
+ * elements apart in qkv.  n_path may be NULL (path_max each).  A path entry
+ * that is not a row (< 0 or >= rows_max) and a position that the ring cannot
+ * hold are skipped. */
+int mb_tree_commit_dev(mb_ctx* ctx, int layer0, int n_layers, int B, int rows_max, const void* qkv,
+                       int qkv_dtype, int64_t qkv_stride, int64_t layer_stride,
+                       const int32_t* pos0, int path_max, const int32_t* path,
+                       const int32_t* n_path);
+
+/* The choice of a beam search's step: for each of B voices, the n_out best of
+ * the continuations of its `width` beams by one id of `vocab`,
+ *   c(w, v) = scores[b][w] + log_softmax(z[b][w])[v],
+ * logits [B][width][vocab].  z are the logits, or with seen (bit v % 32 of
+ * seen[b][w][v / 32]; ceil(vocab / 32) words) the penalised ones: a seen id's
+ * logit is multiplied by the penalty when negative and divided when not, in
+ * fp32 with the penalty rounded to fp32 (MB_PENALTY_F32's arithmetic).  A beam
+ * with done[b][w] != 0 goes on as it is: its one continuation is end_id with
+ * c = scores[b][w] (its logits are not read).  c is formed and compared in
+ * double; ties go to the lower beam, then the higher logit, then the lower id.
+ * A NaN or -inf logit is never chosen, nor a beam whose score is NaN or -inf;
+ * +inf logits share the whole probability.  For k < n_out, best first:
+ *   scores_out[b][k] = c (fp32), parent[b][k] = w, token[b][k] = v,
+ *   done_out[b][k] = 1 when v == end_id (may be NULL),
+ *   seen_out[b][k] = seen[b][w] with v added (may be NULL).
+ * Where fewer continuations exist: -inf, -1, -1, 1 and an empty set.
+ * width and n_out are 1 .. 32.  done may be NULL (none), and then end_id may
+ * be -1 (no id ends a beam); seen may be NULL (no penalty), and then seen_out
+ * is NULL.  Outputs may not be the inputs. */
+int mb_beam_select(mb_ctx* ctx, int B, int width, int vocab, int n_out, const float* logits,
+                   const float* scores, const int32_t* done, int32_t end_id, const uint32_t* seen,
+                   double penalty, float* scores_out, int32_t* parent, int32_t* token,
+                   int32_t* done_out, uint32_t* seen_out);
+/* Bytes of the workspace that mb_beam_select_dev takes (0: none). */
+int mb_beam_select_work(mb_ctx* ctx, int B, int width, int vocab, int n_out, int64_t* bytes);
+/* Device-pointer form (enqueue only): logits of either dtype, rows
+ * logits_stride elements apart.  The workspace as for mb_tree_attention_dev. */
+int mb_beam_select_dev(mb_ctx* ctx, int B, int width, int vocab, int n_out, const void* logits,
+                       int logits_dtype, int64_t logits_stride, const float* scores,
+                       const int32_t* done, int32_t end_id, const uint32_t* seen, double penalty,
+                       float* scores_out, int32_t* parent, int32_t* token, int32_t* done_out,
+                       uint32_t* seen_out, void* work, int64_t work_bytes);
+
+/* Move the rings of n_layers layers from layer0 on to the beams that go on:
+ * sequences 0 .. B-1 are groups of `width` consecutive ones (1 .. 32; B a
+ * multiple of it), and sequence g * width + w takes the slots of sequence
+ * g * width + parent[g * width + w] -- K, V and stored positions, as they were
+ * before the call, for all w at once -- that hold positions pos_from[g] ..
+ * pos_to[g] - 1 (at most capacity of them).  A parent outside [0, width), as
+ * mb_beam_select's -1, leaves its sequence as it is.  pos_from and pos_to are
+ * [B / width]; both NULL: every slot.  Rows that the beams of a group share (a
+ * common prompt's) need not be moved. */
+int mb_ring_reorder(mb_ctx* ctx, int layer0, int n_layers, int B, int width, const int32_t* parent,
+                    const int32_t* pos_from, const int32_t* pos_to);
+/* Device-pointer form (enqueue only); max_rows bounds every pos_to - pos_from
+ * (pass capacity when unknown): it sizes the launch. */
+int mb_ring_reorder_dev(mb_ctx* ctx, int layer0, int n_layers, int B, int width,
+                        const int32_t* parent, const int32_t* pos_from, const int32_t* pos_to,
+                        int32_t max_rows);
+
 /* ------------------------------------------------------------------ model
  * The decoder around the rings, fp32 weights uploaded with mb_upload_tensor.
  * Row ids are int32 [17]: text id in column 0 (< vocab), audio codes in

@@ -39,7 +39,10 @@ EXPORTS = (
     "mb_local_steps", "mb_local_logits", "mb_clear_seen", "mb_decode_step_dev", "mb_local_frame_dev",
     "mb_linear_dev", "mb_split_weights_dev", "mb_linear_split_dev", "mb_linear_noalloc_dev", "mb_decode_frames_dev", "mb_decode_frames", "mb_append_attend",
     "mb_append_attend_dev", "mb_codec_init", "mb_codec_reset", "mb_codec_decode",
-    "mb_codec_decode_dev", "mb_codec_read_ring",
+    "mb_codec_decode_dev", "mb_codec_read_ring", "mb_ring_view", "mb_tree_attention",
+    "mb_tree_attention_work", "mb_tree_attention_dev", "mb_tree_commit", "mb_tree_commit_dev",
+    "mb_beam_select", "mb_beam_select_work", "mb_beam_select_dev", "mb_ring_reorder",
+    "mb_ring_reorder_dev",
 )
 
 
@@ -135,6 +138,25 @@ def load():
         "mb_append_attend": ([_vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp], C.c_int),
         "mb_append_attend_dev": ([_vp, C.c_int, C.c_int, _vp, C.c_int, _i64, _vp, _i32, _vp, _i64,
                                   _vp, _i64], C.c_int),
+        "mb_ring_view": ([_vp, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp)], C.c_int),
+        "mb_tree_attention": ([_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp], C.c_int),
+        "mb_tree_attention_work": ([_vp, C.c_int, C.c_int, _i32, C.POINTER(_i64)], C.c_int),
+        "mb_tree_attention_dev": ([_vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _i64, _vp, _vp,
+                                   _vp, _i32, _vp, _i64, _vp, _i64], C.c_int),
+        "mb_tree_commit": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, _vp],
+                           C.c_int),
+        "mb_tree_commit_dev": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _i64, _i64,
+                                _vp, C.c_int, _vp, _vp], C.c_int),
+        "mb_beam_select": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _i32, _vp,
+                            C.c_double, _vp, _vp, _vp, _vp, _vp], C.c_int),
+        "mb_beam_select_work": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_i64)],
+                                C.c_int),
+        "mb_beam_select_dev": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _i64, _vp,
+                                _vp, _i32, _vp, C.c_double, _vp, _vp, _vp, _vp, _vp, _vp, _i64],
+                               C.c_int),
+        "mb_ring_reorder": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp], C.c_int),
+        "mb_ring_reorder_dev": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _i32],
+                                C.c_int),
         "mb_codec_init": ([_vp, C.POINTER(CodecConfig)], C.c_int),
         "mb_codec_reset": ([_vp, C.c_int, _vp], C.c_int),
         "mb_codec_decode": ([_vp, C.c_int, C.c_int, _vp, _vp], C.c_int),
@@ -159,6 +181,17 @@ def _f32c(a):
 
 def _i32c(a):
     return np.ascontiguousarray(a, dtype=np.int32)
+
+
+class DeviceArray:
+    """Device memory of a context as `__cuda_array_interface__` describes it
+    (torch.as_tensor(a, device="cuda") is a view of it; bf16 comes as int16).
+    Holds the context."""
+
+    def __init__(self, ctx, ptr, shape, typestr):
+        self.ctx = ctx
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr,
+                                         "data": (ptr, False), "strides": None, "version": 3}
 
 
 class Context:
@@ -327,6 +360,122 @@ class Context:
                               q_dtype=MB_DT_F32):
         self.check(self.lib.mb_prefill_attention_dev(self.h, layer, B, rows_max, q_ptr, q_dtype,
                                                      pos0_ptr, n_ptr, out_ptr))
+
+    # -- several hypotheses per voice: drafted trees, beams
+    def ring_view(self):
+        """(K, V, slot_pos) as DeviceArrays: [n_layers][max_seqs][12][capacity][64]
+        fp32 (int16 bits in bf16 contexts) and [n_layers][max_seqs][capacity]
+        int32, the rings themselves."""
+        p = [_vp(), _vp(), _vp()]
+        self.check(self.lib.mb_ring_view(self.h, *(C.byref(x) for x in p)))
+        c = self.cfg
+        kv = "<i2" if c.kv_dtype == MB_KV_BF16 else "<f4"
+        shape = (c.n_layers, c.max_seqs, H, c.capacity, HD)
+        return (DeviceArray(self, p[0].value, shape, kv), DeviceArray(self, p[1].value, shape, kv),
+                DeviceArray(self, p[2].value, (c.n_layers, c.max_seqs, c.capacity), "<i4"))
+
+    def tree_attention(self, layer: int, qkv: np.ndarray, parent, pos0, n_nodes,
+                       out: np.ndarray | None = None) -> np.ndarray:
+        """qkv [B][R][2304], parent [B][R], pos0 [B], n_nodes [B] -> [B][R][768];
+        rows past a sequence's nodes stay as `out` has them (zero without it)."""
+        qkv, parent, pos0, n = _f32c(qkv), _i32c(parent), _i32c(pos0), _i32c(n_nodes)
+        B, R = qkv.shape[0], qkv.shape[1]
+        if qkv.shape != (B, R, QKV) or parent.shape != (B, R) or pos0.shape != (B,) or n.shape != (B,):
+            raise ValueError("tree_attention: shapes do not belong together")
+        if out is None:
+            out = np.zeros((B, R, D), np.float32)
+        elif out.shape != (B, R, D) or out.dtype != np.float32 or not out.flags.c_contiguous:
+            raise ValueError("tree_attention: out is no contiguous float32 [B][R][768]")
+        self.check(self.lib.mb_tree_attention(self.h, layer, B, R, _ptr(qkv), _ptr(parent),
+                                              _ptr(pos0), _ptr(n), _ptr(out)))
+        return out
+
+    def tree_attention_work(self, B: int, rows_max: int, max_pos: int) -> int:
+        """Bytes of tree_attention_dev's workspace."""
+        n = _i64(0)
+        self.check(self.lib.mb_tree_attention_work(self.h, B, rows_max, max_pos, C.byref(n)))
+        return n.value
+
+    def tree_attention_dev(self, layer, B, rows_max, qkv_ptr, parent_ptr, pos0_ptr, n_ptr, max_pos,
+                           out_ptr, work_ptr=None, work_bytes=0, qkv_dtype=MB_DT_F32,
+                           qkv_stride=QKV, out_stride=D):
+        self.check(self.lib.mb_tree_attention_dev(self.h, layer, B, rows_max, qkv_ptr, qkv_dtype,
+                                                  qkv_stride, parent_ptr, pos0_ptr, n_ptr, max_pos,
+                                                  out_ptr, out_stride, work_ptr, work_bytes))
+
+    def tree_commit(self, layer0: int, qkv: np.ndarray, pos0, path, n_path):
+        """qkv [L][B][R][2304] of layers layer0 .. layer0 + L - 1, pos0 [B],
+        path [B][P], n_path [B]: the path's rows go into the rings."""
+        qkv, pos0, path, n = _f32c(qkv), _i32c(pos0), _i32c(path), _i32c(n_path)
+        L, B, R = qkv.shape[:3]
+        if qkv.shape != (L, B, R, QKV) or path.ndim != 2 or len(path) != B or \
+                pos0.shape != (B,) or n.shape != (B,):
+            raise ValueError("tree_commit: shapes do not belong together")
+        self.check(self.lib.mb_tree_commit(self.h, layer0, L, B, R, _ptr(qkv), _ptr(pos0),
+                                           path.shape[1], _ptr(path), _ptr(n)))
+
+    def tree_commit_dev(self, layer0, n_layers, B, rows_max, qkv_ptr, pos0_ptr, path_max, path_ptr,
+                        n_path_ptr, qkv_dtype=MB_DT_F32, qkv_stride=QKV, layer_stride=None):
+        if layer_stride is None:
+            layer_stride = B * rows_max * qkv_stride
+        self.check(self.lib.mb_tree_commit_dev(self.h, layer0, n_layers, B, rows_max, qkv_ptr,
+                                               qkv_dtype, qkv_stride, layer_stride, pos0_ptr,
+                                               path_max, path_ptr, n_path_ptr))
+
+    def beam_select(self, logits: np.ndarray, scores, n_out: int, done=None, end_id: int = -1,
+                    seen=None, penalty: float = 1.2):
+        """logits [B][W][V], scores [B][W] (done [B][W], seen uint32
+        [B][W][ceil(V / 32)]) -> (scores, parent, token, done, seen or None) of
+        the n_out best continuations, each [B][n_out]."""
+        logits, scores = _f32c(logits), _f32c(scores)
+        B, W, V = logits.shape
+        words = (V + 31) // 32
+        done = None if done is None else _i32c(done)
+        seen = None if seen is None else np.ascontiguousarray(seen, dtype=np.uint32)
+        if scores.shape != (B, W) or (done is not None and done.shape != (B, W)) or \
+                (seen is not None and seen.shape != (B, W, words)):
+            raise ValueError("beam_select: shapes do not belong together")
+        so = np.zeros((B, n_out), np.float32)
+        parent, token, done_out = (np.zeros((B, n_out), np.int32) for _ in range(3))
+        seen_out = None if seen is None else np.zeros((B, n_out, words), np.uint32)
+        self.check(self.lib.mb_beam_select(self.h, B, W, V, n_out, _ptr(logits), _ptr(scores),
+                                           _ptr(done), end_id, _ptr(seen), penalty, _ptr(so),
+                                           _ptr(parent), _ptr(token), _ptr(done_out),
+                                           _ptr(seen_out)))
+        return so, parent, token, done_out, seen_out
+
+    def beam_select_work(self, B: int, width: int, vocab: int, n_out: int) -> int:
+        """Bytes of beam_select_dev's workspace."""
+        n = _i64(0)
+        self.check(self.lib.mb_beam_select_work(self.h, B, width, vocab, n_out, C.byref(n)))
+        return n.value
+
+    def beam_select_dev(self, B, width, vocab, n_out, logits_ptr, scores_ptr, scores_out_ptr,
+                        parent_ptr, token_ptr, work_ptr=None, work_bytes=0, logits_dtype=MB_DT_F32,
+                        logits_stride=None, done_ptr=None, end_id=-1, seen_ptr=None, penalty=1.2,
+                        done_out_ptr=None, seen_out_ptr=None):
+        self.check(self.lib.mb_beam_select_dev(
+            self.h, B, width, vocab, n_out, logits_ptr, logits_dtype,
+            vocab if logits_stride is None else logits_stride, scores_ptr, done_ptr, end_id,
+            seen_ptr, penalty, scores_out_ptr, parent_ptr, token_ptr, done_out_ptr, seen_out_ptr,
+            work_ptr, work_bytes))
+
+    def ring_reorder(self, layer0: int, n_layers: int, parent, pos_from=None, pos_to=None):
+        """parent [groups][width]: sequence g * width + w takes the rings of
+        g * width + parent[g][w], at positions pos_from[g] .. pos_to[g] - 1
+        (both None: every slot)."""
+        parent = _i32c(parent)
+        G, W = parent.shape
+        a = None if pos_from is None else _i32c(pos_from)
+        z = None if pos_to is None else _i32c(pos_to)
+        if any(x is not None and x.shape != (G,) for x in (a, z)):
+            raise ValueError("ring_reorder: pos_from and pos_to are [groups]")
+        self.check(self.lib.mb_ring_reorder(self.h, layer0, n_layers, G * W, W, _ptr(parent),
+                                            _ptr(a), _ptr(z)))
+
+    def ring_reorder_dev(self, layer0, n_layers, B, width, parent_ptr, from_ptr, to_ptr, max_rows):
+        self.check(self.lib.mb_ring_reorder_dev(self.h, layer0, n_layers, B, width, parent_ptr,
+                                                from_ptr, to_ptr, max_rows))
 
     # -- the codec decoder
     def codec_init(self, max_voices: int, layers=CODEC_LAYERS, context=CODEC_CONTEXT,

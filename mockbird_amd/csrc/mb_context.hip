@@ -194,6 +194,69 @@ int check_common(mb_ctx* ctx, int layer, int B) {
   return MB_OK;
 }
 
+int check_layers(mb_ctx* ctx, int layer0, int n_layers, int B) {
+  const int rc = check_common(ctx, layer0, B);
+  if (rc) return rc;
+  if (n_layers < 0 || n_layers > ctx->cfg.n_layers - layer0)
+    return fail(ctx, MB_ERR_ARG, "%d layers from %d on, of %d", n_layers, layer0, ctx->cfg.n_layers);
+  return MB_OK;
+}
+
+int check_tree(mb_ctx* ctx, int layer0, int n_layers, int B, int rows_max) {
+  const int rc = check_layers(ctx, layer0, n_layers, B);
+  if (rc) return rc;
+  if (rows_max < 1 || rows_max > kTreeMaxNodes)
+    return fail(ctx, MB_ERR_ARG, "rows_max %d out of [1, %d]", rows_max, kTreeMaxNodes);
+  return MB_OK;
+}
+
+int check_groups(mb_ctx* ctx, int layer0, int n_layers, int B, int width, const void* pos_from,
+                 const void* pos_to) {
+  const int rc = check_layers(ctx, layer0, n_layers, B);
+  if (rc) return rc;
+  if (width < 1 || width > kBeamMax || B % width)
+    return fail(ctx, MB_ERR_ARG, "width %d out of [1, %d], or not a divisor of B %d", width, kBeamMax, B);
+  if (!pos_from != !pos_to) return fail(ctx, MB_ERR_ARG, "pos_from and pos_to come together");
+  return MB_OK;
+}
+
+int check_beam(mb_ctx* ctx, int B, int width, int vocab, int n_out) {
+  if (!ctx) return MB_ERR_ARG;
+  if (B < 0 || width < 1 || width > kBeamMax || n_out < 1 || n_out > kBeamMax)
+    return fail(ctx, MB_ERR_ARG, "B %d voices of %d beams, %d chosen: beams and choices are 1 .. %d", B,
+                width, n_out, kBeamMax);
+  // (ids are int32, with room for one scan past the last)
+  if (vocab < 1 || vocab > (1 << 30)) return fail(ctx, MB_ERR_ARG, "vocab %d out of [1, 2^30]", vocab);
+  return MB_OK;
+}
+
+int check_beam_options(mb_ctx* ctx, int vocab, const void* scores, const void* done, int32_t end_id,
+                       const void* seen, double penalty, const void* scores_out,
+                       const void* done_out, const void* seen_out) {
+  if (end_id < -1 || end_id >= vocab || (done && end_id < 0))
+    return fail(ctx, MB_ERR_ARG, "end_id %d is no id of %d (-1 where no beam is done)", end_id, vocab);
+  if (seen_out && !seen) return fail(ctx, MB_ERR_ARG, "seen_out needs seen");
+  if (seen && (!(penalty > 0.0) || !(penalty < INFINITY)))
+    return fail(ctx, MB_ERR_ARG, "penalty %g is not a positive number", penalty);
+  if ((scores && scores == scores_out) || (done && done == done_out) || (seen && seen == seen_out))
+    return fail(ctx, MB_ERR_ARG, "an output is its input");
+  return MB_OK;
+}
+
+// Rows `stride` elements of e bytes apart start at multiples of 16 bytes.
+bool aligned_rows(const void* p, int64_t stride, int e) {
+  return ((uintptr_t)p & 15) == 0 && (stride * e & 15) == 0;
+}
+
+int check_work(mb_ctx* ctx, const void* work, int64_t bytes, int64_t need) {
+  if (need == 0) return MB_OK;
+  if (!work || bytes < need)
+    return fail(ctx, MB_ERR_ARG, "the workspace holds %lld bytes of %lld", (long long)(work ? bytes : 0),
+                (long long)need);
+  if ((uintptr_t)work & 15) return fail(ctx, MB_ERR_ARG, "the workspace must be 16-byte aligned");
+  return MB_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -591,6 +654,117 @@ int mb_prefill_attention_dev(mb_ctx* ctx, int layer, int B, int rows_max, const 
                                   dense_rows(D, rows_max));
 }
 
+// ------------------------------------------- several hypotheses per voice
+
+int mb_ring_view(mb_ctx* ctx, void** k, void** v, int32_t** slot_pos) {
+  if (!ctx) return MB_ERR_ARG;
+  if (k) *k = ctx->ring_k;
+  if (v) *v = ctx->ring_v;
+  if (slot_pos) *slot_pos = ctx->slot_pos;
+  return MB_OK;
+}
+
+int mb_tree_attention_work(mb_ctx* ctx, int B, int rows_max, int32_t max_pos, int64_t* bytes) {
+  int rc = check_tree(ctx, 0, 1, B, rows_max);
+  if (rc) return rc;
+  if (max_pos < 0) return fail(ctx, MB_ERR_ARG, "max_pos %d is negative", max_pos);
+  if (!bytes) return fail(ctx, MB_ERR_ARG, "null pointer");
+  *bytes = tree_work_bytes(ctx, B, rows_max, max_pos);
+  return MB_OK;
+}
+
+int mb_tree_attention_dev(mb_ctx* ctx, int layer, int B, int rows_max, const void* qkv,
+                          int qkv_dtype, int64_t qkv_stride, const int32_t* parent,
+                          const int32_t* pos0, const int32_t* n_nodes, int32_t max_pos, float* out,
+                          int64_t out_stride, void* work, int64_t work_bytes) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_tree(ctx, layer, 1, B, rows_max);
+  if (rc) return rc;
+  if (qkv_dtype != MB_DT_F32 && qkv_dtype != MB_DT_BF16)
+    return fail(ctx, MB_ERR_ARG, "unknown dtype");
+  if (qkv_stride < QKV || out_stride < D) return fail(ctx, MB_ERR_ARG, "row stride too small");
+  if (max_pos < 0) return fail(ctx, MB_ERR_ARG, "max_pos %d is negative", max_pos);
+  if (!ctx->cfg.wrap && max_pos >= ctx->cfg.capacity)
+    return fail(ctx, MB_ERR_RANGE,
+                "decode position %d exceeds the KV ring (%d slots); it must be sized "
+                "prefill_rows + max_new_frames",
+                max_pos, ctx->cfg.capacity);
+  if (B == 0) return MB_OK;
+  if (!qkv || !parent || !pos0 || !out) return fail(ctx, MB_ERR_ARG, "null pointer");
+  if (!aligned_rows(qkv, qkv_stride, qkv_dtype == MB_DT_BF16 ? 2 : 4) || !aligned_rows(out, out_stride, 4))
+    return fail(ctx, MB_ERR_ARG, "rows must start at multiples of 16 bytes");
+  rc = check_work(ctx, work, work_bytes, tree_work_bytes(ctx, B, rows_max, max_pos));
+  if (rc) return rc;
+  return launch_tree_attention(ctx, global_ring(ctx, layer), B, rows_max, qkv, qkv_dtype, qkv_stride,
+                               parent, pos0, n_nodes, max_pos, out, out_stride, work);
+}
+
+int mb_tree_commit_dev(mb_ctx* ctx, int layer0, int n_layers, int B, int rows_max, const void* qkv,
+                       int qkv_dtype, int64_t qkv_stride, int64_t layer_stride,
+                       const int32_t* pos0, int path_max, const int32_t* path,
+                       const int32_t* n_path) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_tree(ctx, layer0, n_layers, B, rows_max);
+  if (rc) return rc;
+  if (qkv_dtype != MB_DT_F32 && qkv_dtype != MB_DT_BF16)
+    return fail(ctx, MB_ERR_ARG, "unknown dtype");
+  if (qkv_stride < QKV) return fail(ctx, MB_ERR_ARG, "row stride too small");
+  if (path_max < 0) return fail(ctx, MB_ERR_ARG, "path_max %d is negative", path_max);
+  if (B == 0 || n_layers == 0 || path_max == 0) return MB_OK;
+  if (!qkv || !pos0 || !path) return fail(ctx, MB_ERR_ARG, "null pointer");
+  const int e = qkv_dtype == MB_DT_BF16 ? 2 : 4;
+  if (!aligned_rows(qkv, qkv_stride, e) || (n_layers > 1 && !aligned_rows(qkv, layer_stride, e)))
+    return fail(ctx, MB_ERR_ARG, "rows must start at multiples of 16 bytes");
+  if (n_layers > 1 && layer_stride < (int64_t)B * rows_max * qkv_stride)
+    return fail(ctx, MB_ERR_ARG, "layer stride too small");
+  return launch_tree_commit(ctx, layer0, n_layers, B, rows_max, qkv, qkv_dtype, qkv_stride,
+                            layer_stride, pos0, path_max, path, n_path);
+}
+
+int mb_beam_select_work(mb_ctx* ctx, int B, int width, int vocab, int n_out, int64_t* bytes) {
+  int rc = check_beam(ctx, B, width, vocab, n_out);
+  if (rc) return rc;
+  if (!bytes) return fail(ctx, MB_ERR_ARG, "null pointer");
+  *bytes = beam_work_bytes(B, width, vocab, n_out);
+  return MB_OK;
+}
+
+int mb_beam_select_dev(mb_ctx* ctx, int B, int width, int vocab, int n_out, const void* logits,
+                       int logits_dtype, int64_t logits_stride, const float* scores,
+                       const int32_t* done, int32_t end_id, const uint32_t* seen, double penalty,
+                       float* scores_out, int32_t* parent, int32_t* token, int32_t* done_out,
+                       uint32_t* seen_out, void* work, int64_t work_bytes) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_beam(ctx, B, width, vocab, n_out);
+  if (rc) return rc;
+  if (logits_dtype != MB_DT_F32 && logits_dtype != MB_DT_BF16)
+    return fail(ctx, MB_ERR_ARG, "unknown dtype");
+  if (logits_stride < vocab) return fail(ctx, MB_ERR_ARG, "row stride too small");
+  rc = check_beam_options(ctx, vocab, scores, done, end_id, seen, penalty, scores_out, done_out, seen_out);
+  if (rc) return rc;
+  if (B == 0) return MB_OK;
+  if (!logits || !scores || !scores_out || !parent || !token)
+    return fail(ctx, MB_ERR_ARG, "null pointer");
+  rc = check_work(ctx, work, work_bytes, beam_work_bytes(B, width, vocab, n_out));
+  if (rc) return rc;
+  return launch_beam_select(ctx, B, width, vocab, n_out, logits, logits_dtype, logits_stride, scores,
+                            done, end_id, seen, penalty, scores_out, parent, token, done_out,
+                            seen_out, work);
+}
+
+int mb_ring_reorder_dev(mb_ctx* ctx, int layer0, int n_layers, int B, int width,
+                        const int32_t* parent, const int32_t* pos_from, const int32_t* pos_to,
+                        int32_t max_rows) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_groups(ctx, layer0, n_layers, B, width, pos_from, pos_to);
+  if (rc) return rc;
+  if (max_rows < 0) return fail(ctx, MB_ERR_ARG, "max_rows %d is negative", max_rows);
+  if (B == 0 || n_layers == 0 || (max_rows == 0 && pos_from)) return MB_OK;
+  if (!parent) return fail(ctx, MB_ERR_ARG, "null pointer");
+  return launch_ring_reorder(ctx, layer0, n_layers, B, width, parent, pos_from, pos_to,
+                             pos_from ? max_rows : ctx->cfg.capacity);
+}
+
 int mb_linear_dev(mb_ctx* ctx, int M, int N, int K, const float* A, int64_t lda, const float* W,
                   const float* bias, float* C, int64_t ldc, int epi) {
   MB_DEVICE_GUARD(ctx);
@@ -759,6 +933,172 @@ int mb_prefill_attention(mb_ctx* ctx, int layer, int B, int rows_max, const floa
                                 dense_rows(D, rows_max));
   if (rc) return rc;
   MB_HIP(ctx, hipMemcpyAsync(out, d_out, rows * D * 4, hipMemcpyDeviceToHost, ctx->stream));
+  MB_HIP(ctx, sync_stream(ctx));
+  return MB_OK;
+}
+
+int mb_tree_attention(mb_ctx* ctx, int layer, int B, int rows_max, const float* qkv,
+                      const int32_t* parent, const int32_t* pos0, const int32_t* n_nodes, float* out) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_tree(ctx, layer, 1, B, rows_max);
+  if (rc) return rc;
+  if (B == 0) return MB_OK;
+  if (!qkv || !parent || !pos0 || !n_nodes || !out) return fail(ctx, MB_ERR_ARG, "null pointer");
+  int32_t max_pos = 0;
+  for (int b = 0; b < B; b++) {
+    if (n_nodes[b] < 0 || n_nodes[b] > rows_max)
+      return fail(ctx, MB_ERR_ARG, "sequence %d: %d nodes out of [0, %d]", b, n_nodes[b], rows_max);
+    if (pos0[b] < 0 || pos0[b] > INT32_MAX - kTreeMaxNodes)
+      return fail(ctx, MB_ERR_ARG, "sequence %d: position %d out of range", b, pos0[b]);
+    int depth[kTreeMaxNodes];
+    for (int i = 0; i < n_nodes[b]; i++) {
+      const int32_t p = parent[(size_t)b * rows_max + i];
+      if (p < -1 || p >= i)
+        return fail(ctx, MB_ERR_ARG, "sequence %d: parent %d of node %d is no earlier node", b, p, i);
+      depth[i] = p < 0 ? 0 : depth[p] + 1;
+      const int32_t pos = pos0[b] + depth[i];
+      if (!ctx->cfg.wrap && pos >= ctx->cfg.capacity)
+        return fail(ctx, MB_ERR_RANGE,
+                    "decode position %d exceeds the KV ring (%d slots); it must be sized "
+                    "prefill_rows + max_new_frames",
+                    pos, ctx->cfg.capacity);
+      max_pos = std::max(max_pos, pos);
+    }
+  }
+  const size_t rows = (size_t)B * rows_max;
+  const int64_t need = tree_work_bytes(ctx, B, rows_max, max_pos);
+  float* d_qkv = (float*)scratch(ctx, "qkv", rows * QKV * 4);
+  float* d_out = (float*)scratch(ctx, "out", rows * D * 4);
+  int32_t* d_pos = (int32_t*)scratch(ctx, "pos", ((size_t)B * 2 + rows) * 4);
+  void* d_work = need ? scratch(ctx, "tree_work", (size_t)need) : nullptr;
+  if (!d_qkv || !d_out || !d_pos || (need && !d_work))
+    return fail(ctx, MB_ERR_NOMEM, "staging allocation failed");
+  MB_HIP(ctx, hipMemcpyAsync(d_qkv, qkv, rows * QKV * 4, hipMemcpyHostToDevice, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(d_pos, pos0, (size_t)B * 4, hipMemcpyHostToDevice, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(d_pos + B, n_nodes, (size_t)B * 4, hipMemcpyHostToDevice, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(d_pos + 2 * B, parent, rows * 4, hipMemcpyHostToDevice, ctx->stream));
+  rc = launch_tree_attention(ctx, global_ring(ctx, layer), B, rows_max, d_qkv, MB_DT_F32, QKV,
+                             d_pos + 2 * B, d_pos, d_pos + B, max_pos, d_out, D, d_work);
+  if (rc) return rc;
+  // only the rows that were attended: the others stay as the caller has them
+  for (int b = 0; b < B; b++)
+    if (n_nodes[b])
+      MB_HIP(ctx, hipMemcpyAsync(out + (size_t)b * rows_max * D, d_out + (size_t)b * rows_max * D,
+                                 (size_t)n_nodes[b] * D * 4, hipMemcpyDeviceToHost, ctx->stream));
+  MB_HIP(ctx, sync_stream(ctx));
+  return MB_OK;
+}
+
+int mb_tree_commit(mb_ctx* ctx, int layer0, int n_layers, int B, int rows_max, const float* qkv,
+                   const int32_t* pos0, int path_max, const int32_t* path, const int32_t* n_path) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_tree(ctx, layer0, n_layers, B, rows_max);
+  if (rc) return rc;
+  if (path_max < 0) return fail(ctx, MB_ERR_ARG, "path_max %d is negative", path_max);
+  if (B == 0 || n_layers == 0 || path_max == 0) return MB_OK;
+  if (!qkv || !pos0 || !path || !n_path) return fail(ctx, MB_ERR_ARG, "null pointer");
+  for (int b = 0; b < B; b++) {
+    if (pos0[b] < 0) return fail(ctx, MB_ERR_ARG, "sequence %d: negative position %d", b, pos0[b]);
+    if (n_path[b] < 0 || n_path[b] > path_max)
+      return fail(ctx, MB_ERR_ARG, "sequence %d: a path of %d rows out of [0, %d]", b, n_path[b], path_max);
+    const int64_t last = (int64_t)pos0[b] + n_path[b] - 1;
+    if (last > INT32_MAX - 1) return fail(ctx, MB_ERR_ARG, "sequence %d: position overflow", b);
+    if (!ctx->cfg.wrap && n_path[b] > 0 && last >= ctx->cfg.capacity)
+      return fail(ctx, MB_ERR_RANGE,
+                  "decode position %lld exceeds the KV ring (%d slots); it must be sized "
+                  "prefill_rows + max_new_frames",
+                  (long long)last, ctx->cfg.capacity);
+    for (int i = 0; i < n_path[b]; i++) {
+      const int32_t node = path[(size_t)b * path_max + i];
+      if (node < 0 || node >= rows_max)
+        return fail(ctx, MB_ERR_ARG, "sequence %d: path node %d out of [0, %d)", b, node, rows_max);
+    }
+  }
+  const size_t rows = (size_t)n_layers * B * rows_max;
+  float* d_qkv = (float*)scratch(ctx, "qkv", rows * QKV * 4);
+  int32_t* d_pos = (int32_t*)scratch(ctx, "pos", ((size_t)B * (2 + (size_t)path_max)) * 4);
+  if (!d_qkv || !d_pos) return fail(ctx, MB_ERR_NOMEM, "staging allocation failed");
+  MB_HIP(ctx, hipMemcpyAsync(d_qkv, qkv, rows * QKV * 4, hipMemcpyHostToDevice, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(d_pos, pos0, (size_t)B * 4, hipMemcpyHostToDevice, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(d_pos + B, n_path, (size_t)B * 4, hipMemcpyHostToDevice, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(d_pos + 2 * B, path, (size_t)B * path_max * 4, hipMemcpyHostToDevice, ctx->stream));
+  rc = launch_tree_commit(ctx, layer0, n_layers, B, rows_max, d_qkv, MB_DT_F32, QKV,
+                          (int64_t)B * rows_max * QKV, d_pos, path_max, d_pos + 2 * B, d_pos + B);
+  if (rc) return rc;
+  MB_HIP(ctx, sync_stream(ctx));
+  return MB_OK;
+}
+
+int mb_beam_select(mb_ctx* ctx, int B, int width, int vocab, int n_out, const float* logits,
+                   const float* scores, const int32_t* done, int32_t end_id, const uint32_t* seen,
+                   double penalty, float* scores_out, int32_t* parent, int32_t* token,
+                   int32_t* done_out, uint32_t* seen_out) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_beam(ctx, B, width, vocab, n_out);
+  if (rc) return rc;
+  rc = check_beam_options(ctx, vocab, scores, done, end_id, seen, penalty, scores_out, done_out, seen_out);
+  if (rc) return rc;
+  if (B == 0) return MB_OK;
+  if (!logits || !scores || !scores_out || !parent || !token)
+    return fail(ctx, MB_ERR_ARG, "null pointer");
+  const size_t rows = (size_t)B * width, outs = (size_t)B * n_out, words = ((size_t)vocab + 31) / 32;
+  const int64_t need = beam_work_bytes(B, width, vocab, n_out);
+  float* d_logits = (float*)scratch(ctx, "beam_logits", rows * vocab * 4);
+  // scores and done, then the outputs
+  int32_t* d_in = (int32_t*)scratch(ctx, "beam_in", rows * 8);
+  int32_t* d_out = (int32_t*)scratch(ctx, "beam_out", outs * 16);
+  uint32_t* d_seen = seen ? (uint32_t*)scratch(ctx, "beam_seen", (rows + outs) * words * 4) : nullptr;
+  void* d_work = need ? scratch(ctx, "beam_work", (size_t)need) : nullptr;
+  if (!d_logits || !d_in || !d_out || (seen && !d_seen) || (need && !d_work))
+    return fail(ctx, MB_ERR_NOMEM, "staging allocation failed");
+  MB_HIP(ctx, hipMemcpyAsync(d_logits, logits, rows * vocab * 4, hipMemcpyHostToDevice, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(d_in, scores, rows * 4, hipMemcpyHostToDevice, ctx->stream));
+  if (done) MB_HIP(ctx, hipMemcpyAsync(d_in + rows, done, rows * 4, hipMemcpyHostToDevice, ctx->stream));
+  if (seen) MB_HIP(ctx, hipMemcpyAsync(d_seen, seen, rows * words * 4, hipMemcpyHostToDevice, ctx->stream));
+  uint32_t* d_seen_out = seen_out ? d_seen + rows * words : nullptr;
+  rc = launch_beam_select(ctx, B, width, vocab, n_out, d_logits, MB_DT_F32, vocab, (float*)d_in,
+                          done ? d_in + rows : nullptr, end_id, d_seen, penalty, (float*)d_out,
+                          d_out + outs, d_out + 2 * outs, d_out + 3 * outs, d_seen_out, d_work);
+  if (rc) return rc;
+  MB_HIP(ctx, hipMemcpyAsync(scores_out, d_out, outs * 4, hipMemcpyDeviceToHost, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(parent, d_out + outs, outs * 4, hipMemcpyDeviceToHost, ctx->stream));
+  MB_HIP(ctx, hipMemcpyAsync(token, d_out + 2 * outs, outs * 4, hipMemcpyDeviceToHost, ctx->stream));
+  if (done_out)
+    MB_HIP(ctx, hipMemcpyAsync(done_out, d_out + 3 * outs, outs * 4, hipMemcpyDeviceToHost, ctx->stream));
+  if (seen_out)
+    MB_HIP(ctx, hipMemcpyAsync(seen_out, d_seen_out, outs * words * 4, hipMemcpyDeviceToHost, ctx->stream));
+  MB_HIP(ctx, sync_stream(ctx));
+  return MB_OK;
+}
+
+int mb_ring_reorder(mb_ctx* ctx, int layer0, int n_layers, int B, int width, const int32_t* parent,
+                    const int32_t* pos_from, const int32_t* pos_to) {
+  MB_DEVICE_GUARD(ctx);
+  int rc = check_groups(ctx, layer0, n_layers, B, width, pos_from, pos_to);
+  if (rc) return rc;
+  if (B == 0 || n_layers == 0) return MB_OK;
+  if (!parent) return fail(ctx, MB_ERR_ARG, "null pointer");
+  const int G = B / width;
+  int64_t most = pos_from ? 0 : ctx->cfg.capacity;
+  for (int g = 0; pos_from && g < G; g++) {
+    if (pos_from[g] < 0 || pos_to[g] < pos_from[g])
+      return fail(ctx, MB_ERR_ARG, "group %d: positions %d .. %d", g, pos_from[g], pos_to[g]);
+    if (!ctx->cfg.wrap && pos_to[g] > ctx->cfg.capacity)
+      return fail(ctx, MB_ERR_RANGE, "group %d: positions up to %d in a ring of %d slots", g, pos_to[g],
+                  ctx->cfg.capacity);
+    most = std::max<int64_t>(most, pos_to[g] - pos_from[g]);
+  }
+  if (most == 0) return MB_OK;
+  int32_t* d = (int32_t*)scratch(ctx, "pos", ((size_t)B + 2 * G) * 4);
+  if (!d) return fail(ctx, MB_ERR_NOMEM, "staging allocation failed");
+  MB_HIP(ctx, hipMemcpyAsync(d, parent, (size_t)B * 4, hipMemcpyHostToDevice, ctx->stream));
+  if (pos_from) {
+    MB_HIP(ctx, hipMemcpyAsync(d + B, pos_from, (size_t)G * 4, hipMemcpyHostToDevice, ctx->stream));
+    MB_HIP(ctx, hipMemcpyAsync(d + B + G, pos_to, (size_t)G * 4, hipMemcpyHostToDevice, ctx->stream));
+  }
+  rc = launch_ring_reorder(ctx, layer0, n_layers, B, width, d, pos_from ? d + B : nullptr,
+                           pos_from ? d + B + G : nullptr, most);
+  if (rc) return rc;
   MB_HIP(ctx, sync_stream(ctx));
   return MB_OK;
 }

@@ -344,6 +344,31 @@ int launch_window_attention(mb_ctx* ctx, const RingView& ring, int B, int rows_m
                             const float* qkv, const Rows& qkv_rows, const int32_t* pos0,
                             const int32_t* n_rows, float* out, const Rows& out_rows,
                             float* part = nullptr, bool stream = false);
+
+// Attention of drafted trees over the ring and the commit of accepted paths
+// (tree.hip).  `work` holds tree_work_bytes bytes (none where that is 0).
+constexpr int kTreeMaxNodes = 64;
+int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t max_pos);
+int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, const void* qkv,
+                          int qkv_dtype, int64_t qkv_stride, const int32_t* parent,
+                          const int32_t* pos0, const int32_t* n_nodes, int32_t max_pos, float* out,
+                          int64_t out_stride, void* work);
+int launch_tree_commit(mb_ctx* ctx, int layer0, int n_layers, int B, int rows, const void* qkv,
+                       int qkv_dtype, int64_t qkv_stride, int64_t layer_stride, const int32_t* pos0,
+                       int path_max, const int32_t* path, const int32_t* n_path);
+
+// Beam choice and the rings' move to the chosen beams (beam.hip).  `work`
+// holds beam_work_bytes bytes (none where that is 0).
+constexpr int kBeamMax = 32;  // beams of a voice, and continuations chosen
+int64_t beam_work_bytes(int B, int W, int V, int n);
+int launch_beam_select(mb_ctx* ctx, int B, int W, int V, int n, const void* logits, int logits_dtype,
+                       int64_t logits_stride, const float* scores, const int32_t* done,
+                       int32_t end_id, const uint32_t* seen, double penalty, float* scores_out,
+                       int32_t* parent, int32_t* token, int32_t* done_out, uint32_t* seen_out,
+                       void* work);
+int launch_ring_reorder(mb_ctx* ctx, int layer0, int n_layers, int B, int W, const int32_t* parent,
+                        const int32_t* from, const int32_t* to, int64_t max_rows);
+
 int launch_fill_i32(mb_ctx* ctx, int32_t* p, int64_t n, int32_t value);
 // the first n words of `rows` rows, `stride` words apart
 int launch_fill_rows_i32(mb_ctx* ctx, int32_t* p, int rows, int64_t stride, int64_t n, int32_t value);

@@ -1,0 +1,640 @@
+// Attention of drafted trees over the KV rings, and the commit of an accepted
+// path into them.
+//
+// A tree of n <= 64 drafted rows hangs below the last cached position pos0 - 1
+// of a sequence: node i has a parent before it (or none), stands at position
+// p_i = pos0 + depth(i) and sees
+//   - the ring slots whose stored position p satisfies 0 <= p < pos0 and
+//     p_i - p < C: what the window would hold had its ancestors been appended
+//     (their appends evict exactly the positions p <= p_i - C), and nothing of
+//     an earlier draft that was not kept (p >= pos0);
+//   - the drafted rows of its ancestors and its own, K roped at their own
+//     positions and K and V rounded as the ring stores them.
+// So out_i is what appending i's ancestors and i one after another and then
+// attending would give, for all nodes in one pass over the window.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv_types.h"
+#include "mb_internal.h"
+#include "planes.h"
+#include "rope.h"
+
+namespace mb {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kTreeWaves = 4;  // waves per workgroup
+
+struct TreeIn {
+  const void* qkv;  // [B][rows] fused rows, row_stride elements apart
+  int64_t row_stride;
+  int qkv_bf16, rows;
+  const int32_t *parent, *pos0, *n_nodes;  // [B][rows], [B], [B] or null (all rows)
+  const char *k, *v;
+  const int32_t* sp;
+  int64_t seq_stride;
+  int C;
+  const float2* rope;
+  float* out;
+  int64_t out_stride;
+  float* part;  // splits > 1: [unit][split][rows][PART]
+  int splits;
+};
+
+// Nodes of sequence b that are attended (0: none), and the first position.
+__device__ __forceinline__ int tree_size(const int32_t* pos0, const int32_t* n_nodes, int rows,
+                                         int b, int& p0) {
+  p0 = pos0[b];
+  const int n = n_nodes ? min(n_nodes[b], rows) : rows;
+  return p0 < 0 || p0 > INT32_MAX - kTreeMaxNodes ? 0 : n;
+}
+
+// Lane i: the ancestors of node i, itself among them, one bit each.  Every
+// round doubles the length of chain that a lane's mask covers.  A parent that
+// is not an earlier node counts as none.
+__device__ __forceinline__ uint64_t ancestors(const int32_t* parent, int n, int lane) {
+  int par = lane < n ? parent[lane] : -1;
+  if (par >= lane || par < 0) par = -1;
+  uint64_t mask = 1ull << lane;
+  while (__ballot(par >= 0)) {
+    const int from = par >= 0 ? par : lane;
+    const uint32_t lo = __shfl((uint32_t)mask, from), hi = __shfl((uint32_t)(mask >> 32), from);
+    const int up = __shfl(par, from);
+    mask |= (uint64_t)hi << 32 | lo;
+    par = par >= 0 ? up : -1;
+  }
+  return mask;
+}
+
+// Eight dims of a fused row as floats.
+__device__ __forceinline__ void load_row8(const TreeIn& a, int64_t off, float* x) {
+  if (a.qkv_bf16) load8<true>(a.qkv, off, x);
+  else load8<false>(a.qkv, off, x);
+}
+
+__device__ __forceinline__ void rope8(const float2* tab, int32_t pos, int d0, float* x) {
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    float c, s, a, b;
+    rope_cs(tab, pos, (d0 >> 1) + j, c, s);
+    rope_pair(x[2 * j], x[2 * j + 1], c, s, a, b);
+    x[2 * j] = a;
+    x[2 * j + 1] = b;
+  }
+}
+
+// One element of a K or V row.
+template <bool BF16>
+__device__ __forceinline__ float elem(const char* row, int d) {
+  return BF16 ? bf16_lo(((const uint16_t*)row)[d]) : ((const float*)row)[d];
+}
+
+// One workgroup per (sequence, head, split).  A wave takes batches of SB slots
+// (8 KB of K and V) in turn with the other waves of its (sequence, head),
+// forms the scores of all nodes, 16 to a tile, and keeps its own softmax state
+// per node; the waves' states are joined in LDS at the end, and those of
+// several workgroups by k_tree_merge.
+//
+// Scores are formed as S^T = K Q^T, 16 slots x 16 nodes: lane (c = lane % 16,
+// g = lane / 16) of the accumulator holds slots 4g .. 4g + 3 of node c, which is
+// the layout in which the next product O^T = V^T P^T takes P^T, so nothing
+// passes between lanes but the nodes' maxima.
+//  - bf16 rings: v_mfma_f32_16x16x32_bf16, a batch of 32 slots.  q and the
+//    weights are three bf16 planes each (split3), so the products are fp32
+//    products of the bf16 K and V.  Lane (c, g) holds V of its 8 slots at dims
+//    4c .. 4c + 3 (eight 8-byte loads, whole rows of 128 B per instruction), and a
+//    byte permute makes them the four V^T operands of dims 4c + dt.
+//  - fp32 rings: v_mfma_f32_16x16x4_f32, a batch of 16 slots, every operand as
+//    it is loaded (16 bytes a lane).
+// In both, lane (c, g) ends with dims 16g .. 16g + 15 of node c.
+//
+// The next batch's K is loaded once the scores are formed, its V once the
+// weights are applied, so a wave always has half a batch under way.
+//
+// A batch whose slots are all live for every node needs no test per slot; one
+// ballot of the stored positions finds that out.
+//
+// Infinities and NaN: a product of a weight 0 with a V that is not finite, a
+// plane of an infinite q, and a difference of infinities are NaN where the sum
+// over the seen slots alone may not be.  Where anything that is not finite
+// comes out, the workgroup takes its rows again one node at a time, leaving
+// unseen slots out (exact_rows).
+template <bool KV_BF16, int NT>
+struct TreeState {
+  f32x4_t o[NT][4];  // dims 16g + 4i + dt of node c: o[t][dt][i]
+  float m[NT], l[NT];
+};
+
+template <bool KV_BF16>
+struct TreeBatch {
+  u32x4_t k[4];                                           // bf16: [u][h]; fp32: [q]
+  std::conditional_t<KV_BF16, u32x2_t, u32x4_t> v[KV_BF16 ? 8 : 4];
+};
+
+// The same rows again, for inputs that are not finite: lane = slot for the
+// scores, lane = dim for the sums.
+template <bool KV_BF16>
+__device__ __forceinline__ void exact_rows(const TreeIn& a, int b, int head, int split, int unit, int n,
+                                        int p0, uint64_t anc, const char* dk, const char* dv,
+                                        int dpitch) {
+  constexpr int E = KV_BF16 ? 2 : 4, SB = KV_BF16 ? 32 : 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nvalid = min(p0, a.C);
+  const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
+  const char *kb = a.k + off, *vb = a.v + off;
+  const int32_t* sp = a.sp + (int64_t)b * a.C;
+  for (int node = wave; node < n; node += kTreeWaves) {
+    const uint64_t mine = __shfl((uint64_t)anc, node);
+    const int pos = p0 + __popcll(mine) - 1;
+    const int64_t qoff = ((int64_t)b * a.rows + node) * a.row_stride + head * HD + lane;
+    const float x = a.qkv_bf16 ? bf16_lo(((const uint16_t*)a.qkv)[qoff]) : ((const float*)a.qkv)[qoff];
+    const float y = __shfl_xor(x, 1);
+    float c, s, r0, r1;
+    rope_cs(a.rope, pos, lane >> 1, c, s);
+    rope_pair(lane & 1 ? y : x, lane & 1 ? x : y, c, s, r0, r1);
+    const float q = (lane & 1 ? r1 : r0) * 0.125f;
+    float m = -INFINITY, l = 0.f, acc = 0.f;
+    auto rows = [&](const char* kr, const char* vr, int64_t pitch, bool live) {
+      float dot = 0.f;
+      for (int d = 0; d < HD; d++) {
+        const float qd = __shfl(q, d);
+        if (live) dot = fmaf(qd, elem<KV_BF16>(kr + lane * pitch, d), dot);
+      }
+      float mx = live ? dot : -INFINITY;
+      for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+      mx = fmaxf(mx, m);
+      const float at = mx == -INFINITY ? 0.f : mx;
+      const float w = live ? __expf(dot - at) : 0.f, by = __expf(m - at);
+      l = l * by + w;
+      acc *= by;
+      m = mx;
+      const uint64_t who = __ballot(live);
+      for (int j = 0; j < 64; j++) {
+        const float wj = __shfl(w, j);
+        if ((who >> j) & 1) acc = fmaf(wj, elem<KV_BF16>(vr + j * pitch, lane), acc);
+      }
+    };
+    for (int base = split * kTreeWaves * SB; base < nvalid; base += a.splits * kTreeWaves * SB)
+      for (int w0 = 0; w0 < kTreeWaves * SB; w0 += SB) {
+        const int slot = base + w0 + lane;
+        const int p = lane < SB && slot < nvalid ? sp[slot] : -1;
+        const bool live = p >= 0 && p < p0 && (int64_t)pos - p < a.C;
+        if (__ballot(live))
+          rows(kb + (int64_t)(base + w0) * HD * E, vb + (int64_t)(base + w0) * HD * E, HD * E, live);
+      }
+    if (split == 0) rows(dk, dv, dpitch, lane < n && ((mine >> lane) & 1));
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    if (a.splits > 1) {
+      float* pp = a.part + (((int64_t)unit * a.splits + split) * a.rows + node) * PART;
+      pp[lane] = acc;
+      if (lane == 0) {
+        pp[64] = m;
+        pp[65] = l;
+      }
+    } else {
+      a.out[((int64_t)b * a.rows + node) * a.out_stride + head * HD + lane] = l == 0.f ? 0.f : acc / l;
+    }
+  }
+}
+
+template <bool KV_BF16, int NT>
+__global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
+  constexpr int SB = KV_BF16 ? 32 : 16;       // slots per batch
+  constexpr int E = KV_BF16 ? 2 : 4;          // bytes per element
+  constexpr int ROWB = HD * E;                // bytes per slot
+  constexpr int NS = SB / 4;                  // slots of a batch per lane
+  constexpr int NN = NT * 16;
+  constexpr int DR = (NN + SB - 1) / SB * SB; // drafted rows kept, in whole batches
+  constexpr int QP = HD + 4;                  // floats per q row in LDS
+  constexpr int DP = ROWB + 16;               // bytes per drafted row in LDS
+  constexpr int FOLD = kTreeWaves * 16 * PART;
+  __shared__ __align__(16) float sq[NN * QP > FOLD ? NN * QP : FOLD];
+  __shared__ __align__(16) char sdk[DR * DP], sdv[DR * DP];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int unit = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const int b = unit / H, head = unit % H;
+  int p0;
+  const int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
+  if (n <= 0) return;  // the whole workgroup
+  const int c = lane & 15, g = lane >> 4;
+  const int nvalid = min(p0, a.C);
+  const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
+  const char *kb = a.k + off, *vb = a.v + off;
+  const int32_t* sp = a.sp + (int64_t)b * a.C;
+  const int s0 = (split * kTreeWaves + wave) * SB, step = a.splits * kTreeWaves * SB;
+
+  TreeBatch<KV_BF16> x;
+  int32_t spl = -1;
+  // Slots past the window read its last one (slot 0 of an empty window) and
+  // are dead by their position.
+  const int last = max(nvalid - 1, 0);
+  auto load_k = [&](int base) {
+    spl = lane < SB && base + lane < nvalid ? sp[base + lane] : -1;
+    if constexpr (KV_BF16) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const char* r = kb + (int64_t)min(base + 16 * u + c, last) * ROWB + g * 16;
+#pragma unroll
+        for (int h = 0; h < 2; h++) x.k[2 * u + h] = __builtin_nontemporal_load((const u32x4_t*)(r + 64 * h));
+      }
+    } else {
+      const char* r = kb + (int64_t)min(base + c, last) * ROWB + g * 16;
+#pragma unroll
+      for (int q = 0; q < 4; q++) x.k[q] = __builtin_nontemporal_load((const u32x4_t*)(r + 64 * q));
+    }
+  };
+  auto load_v = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < NS; j++) {
+      const char* r = vb + (int64_t)min(base + 16 * (j >> 2) + 4 * g + (j & 3), last) * ROWB + c * 4 * E;
+      if constexpr (KV_BF16) x.v[j] = __builtin_nontemporal_load((const u32x2_t*)r);
+      else x.v[j] = __builtin_nontemporal_load((const u32x4_t*)r);
+    }
+  };
+  load_k(s0);
+  load_v(s0);
+
+  // the nodes' ancestors, and their q (and in the first split K and V) rows
+  const uint64_t anc = ancestors(a.parent + (int64_t)b * a.rows, n, lane);
+  for (int i = threadIdx.x; i < DR * 8; i += 64 * kTreeWaves) {  // whole waves
+    const int node = i >> 3, d0 = (i & 7) * 8, src = min(node, n - 1);
+    const uint32_t lo = __shfl((uint32_t)anc, src), hi = __shfl((uint32_t)(anc >> 32), src);
+    const int32_t pos = p0 + __popc(lo) + __popc(hi) - 1;
+    const int64_t roff = ((int64_t)b * a.rows + src) * a.row_stride + head * HD + d0;
+    float r[8];
+    if (node < NN) {
+      load_row8(a, roff, r);
+      rope8(a.rope, pos, d0, r);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sq[node * QP + d0 + j] = r[j] * 0.125f;  // exact
+    }
+    if (split == 0) {
+      load_row8(a, roff + D, r);
+      rope8(a.rope, pos, d0, r);
+      float w[8];
+      load_row8(a, roff + 2 * D, w);
+      if (node >= n)
+#pragma unroll
+        for (int j = 0; j < 8; j++) r[j] = w[j] = 0.f;
+      store8<KV_BF16>(sdk + node * DP, d0, r);
+      store8<KV_BF16>(sdv + node * DP, d0, w);
+    }
+  }
+  // of the tiles' nodes c: position and ancestors
+  int32_t at[NT];
+  uint64_t sees[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const uint32_t lo = __shfl((uint32_t)anc, 16 * t + c), hi = __shfl((uint32_t)(anc >> 32), 16 * t + c);
+    sees[t] = (uint64_t)hi << 32 | lo;
+    at[t] = p0 + __popcll(sees[t]) - 1;
+  }
+  int deepest = lane < n ? __popcll(anc) - 1 : 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o));
+  __syncthreads();
+
+  // q as the second operand of the scores
+  std::conditional_t<KV_BF16, Planes[NT][2], f32x4_t[NT][4]> q;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const float* r = sq + (16 * t + c) * QP;
+    if constexpr (KV_BF16) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = r[32 * h + 8 * g + j];
+        q[t][h] = split3(v);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) q[t][j] = *(const f32x4_t*)(r + 16 * j + 4 * g);
+    }
+  }
+
+  TreeState<KV_BF16, NT> st;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+#pragma unroll
+    for (int dt = 0; dt < 4; dt++) st.o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    st.m[t] = -INFINITY;
+    st.l[t] = 0.f;
+  }
+
+  // scores s[t][j] of slot 16 (j / 4) + 4g + j % 4 of the batch
+  float s[NT][NS];
+  auto scores = [&]() {
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int u = 0; u < NS / 4; u++) {
+        f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (KV_BF16) {
+#pragma unroll
+          for (int p = 2; p >= 0; p--)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+              d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x.k[2 * u + h]),
+                                                          q[t][h].p[p], d, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[j][e]), q[t][j][e], d, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[t][4 * u + i] = d[i];
+      }
+  };
+  // the batch's scores into the states
+  auto apply = [&]() {
+    bf16x8_t vt[4];
+    if constexpr (KV_BF16) {
+#pragma unroll
+      for (int dt = 0; dt < 4; dt++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          w[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][dt >> 1], x.v[2 * j][dt >> 1],
+                                       dt & 1 ? 0x07060302u : 0x05040100u);
+        vt[dt] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      float mx = s[t][0];
+#pragma unroll
+      for (int j = 1; j < NS; j++) mx = fmaxf(mx, s[t][j]);
+      mx = fmaxf(col_max(mx), st.m[t]);
+      if (__ballot(mx > st.m[t])) {  // uniform
+        const float by = mx == -INFINITY ? 1.f : __expf(st.m[t] - mx);
+        st.l[t] *= by;
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++) st.o[t][dt] *= by;
+        st.m[t] = mx;
+      }
+      const float m = mx == -INFINITY ? 0.f : mx;
+      float p[NS];
+#pragma unroll
+      for (int j = 0; j < NS; j++) {
+        p[j] = __expf(s[t][j] - m);
+        st.l[t] += p[j];
+      }
+      if constexpr (KV_BF16) {
+        const Planes pp = split3(p);
+#pragma unroll
+        for (int k = 2; k >= 0; k--)
+#pragma unroll
+          for (int dt = 0; dt < 4; dt++)
+            st.o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[dt], pp.p[k], st.o[t][dt], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int dt = 0; dt < 4; dt++)
+            st.o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][dt]), p[j],
+                                                               st.o[t][dt], 0, 0, 0);
+      }
+    }
+  };
+
+  for (int base = s0; base < nvalid; base += step) {
+    const int32_t sc = spl;
+    const bool more = base + step < nvalid;
+    scores();
+    if (more) load_k(base + step);
+    const uint64_t all = __ballot(sc >= 0 && sc < p0 && p0 + deepest - sc < a.C);
+    constexpr uint64_t full = (1ull << SB) - 1;
+    if (all != full) {  // uniform
+#pragma unroll
+      for (int j = 0; j < NS; j++) {
+        const int32_t p = __shfl(sc, 16 * (j >> 2) + 4 * g + (j & 3));
+        const bool cached = p >= 0 && p < p0;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+          if (!(cached && at[t] - p < a.C)) s[t][j] = -INFINITY;
+      }
+    }
+    apply();
+    if (more) load_v(base + step);
+  }
+  if (split == 0) {
+    for (int base = wave * SB; base < DR; base += kTreeWaves * SB) {
+      if constexpr (KV_BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          x.k[i] = *(const u32x4_t*)(sdk + (base + 16 * (i >> 1) + c) * DP + g * 16 + 64 * (i & 1));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x.k[i] = *(const u32x4_t*)(sdk + (base + c) * DP + g * 16 + 64 * i);
+      }
+#pragma unroll
+      for (int j = 0; j < NS; j++)
+        x.v[j] = *(const std::remove_reference_t<decltype(x.v[0])>*)(
+            sdv + (base + 16 * (j >> 2) + 4 * g + (j & 3)) * DP + c * 4 * E);
+      scores();
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int j = 0; j < NS; j++) {
+          const int row = base + 16 * (j >> 2) + 4 * g + (j & 3);
+          if (!((sees[t] >> row) & 1)) s[t][j] = -INFINITY;
+        }
+      apply();
+    }
+  }
+
+  // join the waves' states, a tile of 16 nodes at a time
+  bool bad = false;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const float l = col_sum(st.l[t]);
+    __syncthreads();
+    float* f = sq + (wave * 16 + c) * PART;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      *(f32x4_t*)(f + 16 * g + 4 * i) = f32x4_t{st.o[t][0][i], st.o[t][1][i], st.o[t][2][i], st.o[t][3][i]};
+    if (g == 0) {
+      f[64] = st.m[t];
+      f[65] = l;
+    }
+    __syncthreads();
+    const int i = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, node = 16 * t + i;
+    float M = -INFINITY, L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; w++) M = fmaxf(M, sq[(w * 16 + i) * PART + 64]);
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; w++) {
+      const float* r = sq + (w * 16 + i) * PART;
+      const float by = M == -INFINITY ? 0.f : __expf(r[64] - M);
+      L += by * r[65];
+      o += by * *(const f32x4_t*)(r + d);
+    }
+    if (node < n) {
+      bad |= !(fabsf(o[0]) < INFINITY && fabsf(o[1]) < INFINITY && fabsf(o[2]) < INFINITY &&
+               fabsf(o[3]) < INFINITY && fabsf(L) < INFINITY && M < INFINITY);
+      if (a.splits > 1) {
+        float* pp = a.part + (((int64_t)unit * a.splits + split) * a.rows + node) * PART;
+        *(f32x4_t*)(pp + d) = o;
+        if (d == 0) {
+          pp[64] = M;
+          pp[65] = L;
+        }
+      } else {
+        float* op = a.out + ((int64_t)b * a.rows + node) * a.out_stride + head * HD + d;
+        const float by = L == 0.f ? 0.f : 1.f / L;
+        *(f32x4_t*)op = o * by;
+      }
+    }
+  }
+  if (__syncthreads_or(bad))
+    exact_rows<KV_BF16>(a, b, head, split, unit, n, p0, anc, sdk, sdv, DP);
+}
+
+// The states of a window shared by several workgroups: 16 nodes of one
+// (sequence, head) per workgroup.
+__global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a) {
+  const int unit = blockIdx.x, b = unit / H, head = unit % H;
+  int p0;
+  const int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
+  const int node = blockIdx.y * 16 + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
+  if (node >= n) return;
+  const float* r = a.part + ((int64_t)unit * a.splits * a.rows + node) * PART;
+  const int64_t step = (int64_t)a.rows * PART;
+  float M = -INFINITY, L = 0.f;
+  for (int s = 0; s < a.splits; s++) M = fmaxf(M, r[s * step + 64]);
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; s++) {
+    const float m = r[s * step + 64], by = m == -INFINITY ? 0.f : __expf(m - M);
+    const f32x4_t v = *(const f32x4_t*)(r + s * step + d);
+    L += by * r[s * step + 65];
+    o += by * v;
+  }
+  const float by = L == 0.f ? 0.f : 1.f / L;
+  *(f32x4_t*)(a.out + ((int64_t)b * a.rows + node) * a.out_stride + head * HD + d) = o * by;
+}
+
+// Workgroups that share a (sequence, head)'s window: enough to fill the chip,
+// each wave with a batch of its own at least.
+static int tree_splits(const mb_ctx* ctx, int B, int32_t max_pos) {
+  const int64_t units = (int64_t)B * H, sb = ctx->cfg.kv_dtype == MB_KV_BF16 ? 32 : 16;
+  const int64_t window = std::min<int64_t>(std::max(max_pos, 1), ctx->cfg.capacity);
+  const int64_t most = (window + sb * kTreeWaves - 1) / (sb * kTreeWaves);
+  return (int)std::max<int64_t>(1, std::min(most, 768 / units));
+}
+
+int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
+  if (B < 1) return 0;
+  const int s = tree_splits(ctx, B, max_pos);
+  return s > 1 ? (int64_t)B * H * s * rows * PART * 4 : 0;
+}
+
+int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, const void* qkv,
+                          int qkv_dtype, int64_t qkv_stride, const int32_t* parent,
+                          const int32_t* pos0, const int32_t* n_nodes, int32_t max_pos, float* out,
+                          int64_t out_stride, void* work) {
+  TreeIn a;
+  a.qkv = qkv;
+  a.row_stride = qkv_stride;
+  a.qkv_bf16 = qkv_dtype == MB_DT_BF16;
+  a.rows = rows;
+  a.parent = parent;
+  a.pos0 = pos0;
+  a.n_nodes = n_nodes;
+  a.k = (const char*)ring.k;
+  a.v = (const char*)ring.v;
+  a.sp = ring.sp;
+  a.seq_stride = ring.seq_stride;
+  a.C = ring.C;
+  a.rope = ctx->rope_tab;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.part = (float*)work;
+  a.splits = tree_splits(ctx, B, max_pos);
+  const dim3 grid((unsigned)(B * H * a.splits));
+  auto go = [&](auto nt) {
+    constexpr int NT = decltype(nt)::value;
+    if (ring.bf16) hipLaunchKernelGGL((k_tree<true, NT>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((k_tree<false, NT>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
+  };
+  if (rows <= 16) go(std::integral_constant<int, 1>{});
+  else if (rows <= 32) go(std::integral_constant<int, 2>{});
+  else if (rows <= 48) go(std::integral_constant<int, 3>{});
+  else go(std::integral_constant<int, 4>{});
+  MB_HIP(ctx, hipGetLastError());
+  if (a.splits > 1) {
+    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(B * H), (unsigned)((rows + 15) / 16)), dim3(256),
+                       0, ctx->stream, a);
+    MB_HIP(ctx, hipGetLastError());
+  }
+  return MB_OK;
+}
+
+// ----------------------------------------------------------------- commit
+
+// Row i of sequence b's path, node path[b][i] of its drafted rows, goes to
+// position pos0[b] + i of every layer's ring as k_ring_write would write it.
+// Each thread owns 8 dims of one head of one row of one layer; a row that a
+// later one of the same path overwrites is not stored, nor one whose node is
+// not a drafted row or whose position the ring cannot hold.
+template <bool IN_BF16, bool KV_BF16>
+__global__ __launch_bounds__(256) void k_tree_commit(
+    const void* __restrict__ qkv, int64_t row_stride, int64_t layer_stride, int rows,
+    const int32_t* __restrict__ pos0, const int32_t* __restrict__ path, int path_max,
+    const int32_t* __restrict__ n_path, int B, int n_layers, void* __restrict__ ring_k,
+    void* __restrict__ ring_v, int32_t* __restrict__ slot_pos, int64_t seq_stride,
+    int64_t layer_seqs, int C, int wrap, const float2* __restrict__ rope_tab) {
+  const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t row_id = t / (H * 8);
+  if (row_id >= (int64_t)n_layers * B * path_max) return;
+  const int part = (int)(t % (H * 8)), head = part >> 3, d0 = (part & 7) * 8;
+  const int i = (int)(row_id % path_max);
+  const int b = (int)(row_id / path_max % B), layer = (int)(row_id / path_max / B);
+  const int n = min(n_path ? n_path[b] : path_max, path_max);
+  if (i >= n || (n > C && i < n - C)) return;
+  const int node = path[(int64_t)b * path_max + i];
+  const int64_t p64 = (int64_t)pos0[b] + i;
+  if (node < 0 || node >= rows || pos0[b] < 0 || p64 > INT32_MAX || (!wrap && p64 >= C)) return;
+  const int32_t pos = (int32_t)p64;
+  const int slot = wrap ? pos % C : pos;
+  const int64_t roff = layer * layer_stride + ((int64_t)b * rows + node) * row_stride + head * HD + d0;
+  float k[8], v[8];
+  load8<IN_BF16>(qkv, roff + D, k);
+  load8<IN_BF16>(qkv, roff + 2 * D, v);
+  rope8(rope_tab, pos, d0, k);
+  const int64_t seq = layer * layer_seqs + b;
+  const int64_t koff = seq * seq_stride + ((int64_t)head * C + slot) * HD + d0;
+  store8<KV_BF16>(ring_k, koff, k);
+  store8<KV_BF16>(ring_v, koff, v);
+  if (part == 0) slot_pos[seq * C + slot] = pos;
+}
+
+int launch_tree_commit(mb_ctx* ctx, int layer0, int n_layers, int B, int rows, const void* qkv,
+                       int qkv_dtype, int64_t qkv_stride, int64_t layer_stride, const int32_t* pos0,
+                       int path_max, const int32_t* path, const int32_t* n_path) {
+  const int64_t threads = (int64_t)n_layers * B * path_max * H * 8;
+  const int64_t blocks = (threads + 255) / 256;
+  if (blocks > INT32_MAX) return fail(ctx, MB_ERR_ARG, "too many rows in one call");
+  const RingView ring = global_ring(ctx, layer0);
+  auto go = [&](auto in, auto kv) {
+    hipLaunchKernelGGL((k_tree_commit<decltype(in)::value, decltype(kv)::value>), dim3((unsigned)blocks),
+                       dim3(256), 0, ctx->stream, qkv, qkv_stride, layer_stride, rows, pos0, path,
+                       path_max, n_path, B, n_layers, ring.k, ring.v, ring.sp, ring.seq_stride,
+                       (int64_t)ctx->cfg.max_seqs, ring.C, ring.wrap, ctx->rope_tab);
+  };
+  std::true_type yes;
+  std::false_type no;
+  if (qkv_dtype == MB_DT_BF16) { if (ring.bf16) go(yes, yes); else go(yes, no); }
+  else { if (ring.bf16) go(no, yes); else go(no, no); }
+  MB_HIP(ctx, hipGetLastError());
+  return MB_OK;
+}
+
+}  // namespace mb
