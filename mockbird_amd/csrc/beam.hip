@@ -39,10 +39,82 @@ __device__ __forceinline__ uint32_t wave_min(uint32_t x) {
 __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
   return wave_reduce(x, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, (uint64_t)dpp_u32<CTRL>((uint32_t)(u >> 32)) << 32 | dpp_u32<CTRL>((uint32_t)u));
+}
 __device__ __forceinline__ double wave_sum(double x) {
+  x += dpp_f64<0xB1>(x);
+  x += dpp_f64<0x4E>(x);
+  x += dpp_f64<0x141>(x);
+  x += dpp_f64<0x140>(x);
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Integers in the order of the floats (-0 as 0), above 0.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint64_t order_of(double c) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, c + 0.0);
+  return u >> 63 ? ~u : u | (1ull << 63);
+}
+
+// Raises lo, which at_lo >= n of some keys reach, until hardly more than n do, by
+// the counts of keys that reach WAYS - 1 bounds between lo and hi (which no key
+// exceeds).  count(bound) is uniform.  (A step is a chain of compare, count and
+// branch of some 300 cycles whatever WAYS is: by halves 8 steps took 2400.)
+constexpr int kSlack = 8;
+template <int WAYS, class Count>
+__device__ __forceinline__ void raise(uint32_t& lo, int& at_lo, uint32_t hi, int n, Count count) {
+  while (at_lo > n + kSlack && lo < hi) {
+    const uint32_t step = (hi - lo) / WAYS + 1, from = lo;
+    uint32_t k = 0;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+    for (int w = 1; w < WAYS; w++) {
+      const int c = count(from + w * step);
+      if (c >= n) {
+        k = w;
+        at_lo = c;
+      }
+    }
+    lo = from + k * step;
+    hi = min(hi, lo + step - 1);
+  }
+}
+// Lanes of `who` below this one.
+__device__ __forceinline__ int rank_in(uint64_t who) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+}
+// The rank of the lane's key among the 64 in LDS, of which the first `count` may
+// be other than 0, the lower lane first on equal ones (UNIQUE: there are none).
+// Read back as broadcasts, 8 at a time: some 20 cycles a key, where reading lanes
+// into scalar registers took 75.
+template <bool UNIQUE>
+__device__ __forceinline__ int rank_of(const uint64_t* keys, uint64_t key, int count, int lane) {
+  int r = 0;
+  for (int k0 = 0; k0 < count; k0 += 8) {  // uniform
+    ulonglong2 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = ((const ulonglong2*)(keys + k0))[i];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint64_t k = i & 1 ? o[i >> 1].y : o[i >> 1].x;
+      r += k > key || (!UNIQUE && k == key && k0 + i < lane);
+    }
+  }
+  return r;
+}
+// LDS accesses of one wave before and after this one stay in their order.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // ------------------------------------------------------------- one row
@@ -66,9 +138,75 @@ struct RowTop {
   double sum = 0.0;
 };
 
-// Merge 16 values a lane into the list: n rounds of the wave's best.
+// Merge 16 values a lane into the list.  A bound that n lanes' best values reach
+// leaves hardly more than n values; with the list's they are collected in LDS,
+// one to a lane, and ranked by counting.  Where more than 64 reach it the bound is
+// raised by counting values instead of lanes, and where that does not help
+// (equal values) the list is taken in n rounds of the wave's best.
 template <class Id>
-__device__ __forceinline__ void take_top(float (&z)[16], Id id, int n, int lane, RowTop& t) {
+__device__ __forceinline__ void take_top(float (&z)[16], Id id, int n, int lane, uint64_t* buf, RowTop& t) {
+  auto key_of = [](float v, uint32_t id) { return (uint64_t)order_of(v) << 32 | ~id; };
+  float best = z[0];
+#pragma unroll
+  for (int j = 1; j < 16; j++) best = fmaxf(best, z[j]);
+  const bool mine = lane < n && t.id != kNoId;
+  const int listed = __popcll(__ballot(mine));
+  const uint32_t top = order_of(best), held = mine ? order_of(t.v) : 0u;
+  // values up to the list's last can not enter a full list
+  uint32_t lo = 1 + (listed == n ? (uint32_t)__builtin_amdgcn_readlane((int)held, n - 1) : order_of(-INFINITY));
+  const uint32_t hi = wave_umax(top);
+  if (hi < lo) return;  // uniform: nothing enters the list
+  int at_lo = __popcll(__ballot(top >= lo));
+  bool whole = at_lo < n;  // too few for a bound: every value that may enter
+  if (!whole) {
+    lo = wave_min(top >= lo ? top : ~0u);  // (the values in use span few of the keys)
+    raise<8>(lo, at_lo, hi, n, [&](uint32_t k) { return __popcll(__ballot(top >= k)); });
+  }
+  int count = 0, all = 0;
+  for (int pass = 0; pass < 2; pass++) {
+    const float bound = value_of(lo);
+    count = 0;
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      // (every lane stores, what is not taken to place 64: no branches)
+      const bool in = z[j] >= bound;
+      const uint64_t who = __ballot(in);
+      buf[in ? min(count + rank_in(who), 64) : 64] = key_of(z[j], id(j));
+      count += __popcll(who);
+    }
+    const bool in = mine && (whole || held >= lo);
+    const uint64_t who = __ballot(in);
+    buf[in ? min(count + rank_in(who), 64) : 64] = key_of(t.v, t.id);
+    all = count + __popcll(who);
+    if (all <= 64 || pass) break;  // uniform
+    const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)held);  // the list's best
+    whole = false;
+    at_lo = all;
+    if (at_lo > n)
+      raise<2>(lo, at_lo, max(hi, first), n, [&](uint32_t k) {
+        const float v = value_of(k);
+        int c = __popcll(__ballot(held >= k));
+#pragma unroll
+        for (int j = 0; j < 16; j++) c += __popcll(__ballot(z[j] >= v));
+        return c;
+      });
+  }
+  if (all <= 64) {  // uniform
+    wave_order();
+    if (lane >= all) buf[lane] = 0ull;
+    wave_order();
+    uint64_t key = buf[lane];
+    const int r = rank_of<true>(buf, key, all, lane);
+    wave_order();
+    if (lane < all && r < n) buf[r] = key;
+    wave_order();
+    key = buf[lane];
+    wave_order();
+    const bool some = lane < min(n, all);
+    t.v = some ? value_of((uint32_t)(key >> 32)) : -INFINITY;
+    t.id = some ? ~(uint32_t)key : kNoId;
+    return;
+  }
   float nv = -INFINITY;
   uint32_t ni = kNoId;
   for (int r = 0; r < n; r++) {
@@ -82,10 +220,7 @@ __device__ __forceinline__ void take_top(float (&z)[16], Id id, int n, int lane,
       }
     const float top = wave_max(bv);
     if (top == -INFINITY) break;  // uniform
-    const uint64_t who = __ballot(bv == top);
-    const uint32_t win = __popcll(who) == 1
-                             ? (uint32_t)__builtin_amdgcn_readlane((int)bi, __ffsll((unsigned long long)who) - 1)
-                             : wave_min(bv == top ? bi : kNoId);
+    const uint32_t win = wave_min(bv == top ? bi : kNoId);
     if (lane == r) {
       nv = top;
       ni = win;
@@ -103,7 +238,7 @@ __device__ __forceinline__ void take_top(float (&z)[16], Id id, int n, int lane,
 // maximum leaves the whole sum to the ids that reach it.
 template <bool BF16>
 __device__ __forceinline__ void scan_row(const void* row, const uint32_t* seen, float penalty, int lo,
-                                         int hi, int n, int lane, RowTop& t) {
+                                         int hi, int n, int lane, uint64_t* buf, RowTop& t) {
   constexpr int PER = BF16 ? 8 : 4;  // consecutive ids of a lane's load
   float least = -INFINITY;           // the n-th best so far
   for (int base = lo; base < hi; base += kScan) {
@@ -126,14 +261,19 @@ __device__ __forceinline__ void scan_row(const void* row, const uint32_t* seen, 
       }
     }
     if (seen) {  // uniform
+      const double by = 1.0 / (double)penalty;
 #pragma unroll
       for (int q = 0; q < 16 / PER; q++) {
         const int at = (int)id(q * PER);
         const uint32_t bits = at < hi ? seen[at >> 5] >> (at & 31) : 0u;
 #pragma unroll
         for (int e = 0; e < PER; e++) {
+          // (the double product rounds once to the fp32 product, and with the
+          // reciprocal to the fp32 quotient: no quotient of two floats is
+          // within 2^-50 of the middle between two floats)
           float& x = z[q * PER + e];
-          if ((bits >> e) & 1) x = x < 0.f ? x * penalty : x / penalty;
+          const float y = (float)((double)x * (x < 0.f ? (double)penalty : by));
+          x = (bits >> e) & 1 ? y : x;
         }
       }
     }
@@ -150,15 +290,20 @@ __device__ __forceinline__ void scan_row(const void* row, const uint32_t* seen, 
       t.m = mx;
     }
     float p[16];
+    if (t.m < INFINITY) {  // uniform
 #pragma unroll
-    for (int j = 0; j < 16; j++) p[j] = z[j] == t.m ? 1.f : __expf(z[j] - t.m);
+      for (int j = 0; j < 16; j++) p[j] = __expf(z[j] - t.m);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++) p[j] = z[j] == t.m ? 1.f : 0.f;
+    }
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1)
 #pragma unroll
       for (int j = 0; j < w; j++) p[j] += p[j + w];
     t.sum += (double)p[0];
     if (mx > least) {
-      take_top(z, id, n, lane, t);
+      take_top(z, id, n, lane, buf, t);
       least = __shfl(t.v, n - 1);
     }
   }
@@ -190,31 +335,43 @@ __device__ __forceinline__ char* part_row(const BeamIn& a, int64_t row, int chun
   return a.part + (row * a.chunks + chunk) * (int64_t)(sizeof(PartRow) + a.n * 8);
 }
 
-__device__ __forceinline__ void scan(const BeamIn& a, int64_t row, int lo, int hi, int lane, RowTop& t) {
+__device__ __forceinline__ void scan(const BeamIn& a, int64_t row, int lo, int hi, int lane, uint64_t* buf,
+                                     RowTop& t) {
   const char* p = (const char*)a.logits + row * a.stride * (a.bf16 ? 2 : 4);
   const uint32_t* seen = a.seen ? a.seen + row * a.words : nullptr;
-  if (a.bf16) scan_row<true>(p, seen, a.penalty, lo, hi, a.n, lane, t);
-  else scan_row<false>(p, seen, a.penalty, lo, hi, a.n, lane, t);
+  if (a.bf16) scan_row<true>(p, seen, a.penalty, lo, hi, a.n, lane, buf, t);
+  else scan_row<false>(p, seen, a.penalty, lo, hi, a.n, lane, buf, t);
   t.sum = wave_sum(t.sum);
+}
+
+// What a part holds whose row is not looked at.
+__device__ __forceinline__ void part_empty(const BeamIn& a, int64_t row, int chunk, int lane) {
+  char* p = part_row(a, row, chunk);
+  if (lane == 0) *(PartRow*)p = PartRow{0.0, -INFINITY, 0u};
+  if (lane < a.n) ((uint2*)(p + sizeof(PartRow)))[lane] = make_uint2(__float_as_uint(-INFINITY), kNoId);
 }
 
 // A wave per part of a row.
 __global__ __launch_bounds__(256) void k_beam_scan(const BeamIn a, int64_t parts) {
+  __shared__ __align__(16) uint64_t buf[4][66];
   const int lane = threadIdx.x & 63;
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= parts) return;
   const int64_t row = i / a.chunks;
   const int c = (int)(i % a.chunks);
-  if (a.done && a.done[row]) return;  // an ended beam's logits are not looked at
+  if (a.done && a.done[row]) {  // its logits are not looked at
+    part_empty(a, row, c, lane);
+    return;
+  }
   RowTop t;
-  scan(a, row, c * a.chunk, min(a.V, (c + 1) * a.chunk), lane, t);
+  scan(a, row, c * a.chunk, min(a.V, (c + 1) * a.chunk), lane, buf[threadIdx.x >> 6], t);
   char* p = part_row(a, row, c);
   if (lane == 0) *(PartRow*)p = PartRow{t.sum, t.m, 0u};
   if (lane < a.n) ((uint2*)(p + sizeof(PartRow)))[lane] = make_uint2(__float_as_uint(t.v), t.id);
 }
 
 // The parts of a row joined.
-__device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, RowTop& t) {
+__device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, uint64_t* buf, RowTop& t) {
   PartRow h{0.0, -INFINITY, 0u};
   if (lane < a.chunks) h = *(const PartRow*)part_row(a, row, lane);
   t.m = wave_max(h.m);
@@ -222,6 +379,7 @@ __device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, Row
   const double by = h.m == t.m ? 1.0 : (double)__expf(h.m - t.m);
   t.sum = wave_sum(h.sum * by);
   const int all = a.chunks * a.n;
+  const uint32_t per = (1u << 20) / a.n + 1;  // i / n as a product: i < 2^11, n <= 2^5
   for (int base = 0; base < all; base += kScan) {
     float z[16];
     uint32_t ids[16];
@@ -229,104 +387,175 @@ __device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, Row
     for (int j = 0; j < 16; j++) {
       const int i = base + 64 * j + lane;
       uint2 w = make_uint2(__float_as_uint(-INFINITY), kNoId);
-      if (i < all) w = ((const uint2*)(part_row(a, row, i / a.n) + sizeof(PartRow)))[i % a.n];
+      if (i < all) {
+        const int c = (int)(i * per >> 20);
+        w = ((const uint2*)(part_row(a, row, c) + sizeof(PartRow)))[i - c * a.n];
+      }
       z[j] = __uint_as_float(w.x);
       ids[j] = w.y;
     }
-    take_top(z, [&](int j) { return ids[j]; }, a.n, lane, t);
+    take_top(z, [&](int j) { return ids[j]; }, a.n, lane, buf, t);
   }
 }
 
-// A double as an integer of the same order (-0 as 0).
-__device__ __forceinline__ uint64_t order_of(double c) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, c + 0.0);
-  return u >> 63 ? ~u : u | (1ull << 63);
+// The n best of `all` <= 64 J keys in LDS, the lower index first on equal ones,
+// as take_top finds a row's: lane k returns the k-th's index, or -1.
+template <int J>
+__device__ __forceinline__ int best_of(uint64_t* lk, int all, int n, int lane, uint64_t* buf, int32_t* at64) {
+  int count, i = lane;
+  if (J == 1) {
+    count = all;
+  } else {
+    uint32_t hk[J], top = 0u;  // the keys' upper words
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      const int at = 64 * j + lane;
+      hk[j] = at < all ? (uint32_t)(lk[at] >> 32) : 0u;
+      top = max(top, hk[j]);
+    }
+    auto reach = [&](uint32_t k) {
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < J; j++) c += __popcll(__ballot(hk[j] >= k));
+      return c;
+    };
+    uint32_t least = ~0u;
+#pragma unroll
+    for (int j = 0; j < J; j++) least = min(least, hk[j] ? hk[j] : ~0u);
+    const uint32_t hi = wave_umax(top);
+    uint32_t lo = max(1u, min(hi, wave_min(least)));
+    count = reach(lo);
+    raise<4>(lo, count, hi, n, reach);
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      const bool in = hk[j] >= lo;
+      const uint64_t who = __ballot(in);
+      at64[in ? min(at + rank_in(who), 64) : 64] = 64 * j + lane;  // in the index's order
+      at += __popcll(who);
+    }
+    wave_order();
+    if (lane < min(count, 64)) i = at64[lane];
+  }
+  int mine = -1;
+  if (count <= 64) {  // uniform
+    const uint64_t k = lane < count ? lk[i] : 0ull;
+    buf[lane] = k;
+    wave_order();
+    const int r = rank_of<false>(buf, k, count, lane);
+    if (lane < n) at64[lane] = -1;
+    wave_order();
+    if (k && r < n) at64[r] = i;
+    wave_order();
+    if (lane < n) mine = at64[lane];
+    return mine;
+  }
+  for (int r = 0; r < n; r++) {  // many equal keys: n rounds of the wave's best
+    uint64_t bk = 0ull;
+    uint32_t bi = kNoId;
+    for (int at = lane; at < all; at += 64)
+      if (lk[at] > bk) {
+        bk = lk[at];
+        bi = at;
+      }
+    const uint32_t hi = wave_umax((uint32_t)(bk >> 32));
+    if (hi == 0u) break;
+    const uint32_t low = wave_umax((uint32_t)(bk >> 32) == hi ? (uint32_t)bk : 0u);
+    const uint32_t win = wave_min((uint32_t)(bk >> 32) == hi && (uint32_t)bk == low ? bi : kNoId);
+    if (lane == r) mine = (int)win;
+    wave_order();
+    if (bi == win) lk[bi] = 0ull;
+    wave_order();
+  }
+  return mine;
 }
 
 // One workgroup per voice, its waves taking the beams' rows in turn; then the
-// first wave merges the beams' lists, lane w holding the head of beam w's.
+// first wave takes the n best of the W n candidates by c.  On equal c the lower
+// beam goes first and, within a beam, the list's order holds.
 constexpr int kBeamWaves = 16;
 template <bool FUSED>
 __global__ __launch_bounds__(64 * kBeamWaves) void k_beam_pick(const BeamIn a) {
-  __shared__ float lv[kBeamMax][kBeamMax];
-  __shared__ uint32_t li[kBeamMax][kBeamMax];
+  __shared__ float lv[kBeamMax * kBeamMax];
+  __shared__ uint32_t li[kBeamMax * kBeamMax];
   __shared__ float lm[kBeamMax];
-  __shared__ double ls[kBeamMax];
-  __shared__ int32_t from[kBeamMax], tok[kBeamMax];
+  __shared__ double ls[kBeamMax], sc[kBeamMax];
+  __shared__ uint64_t lk[kBeamMax * kBeamMax];
+  __shared__ int32_t from[kBeamMax], tok[kBeamMax], at64[65];
+  __shared__ __align__(16) uint64_t buf[kBeamWaves][66];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int b = blockIdx.x;
+  const int b = blockIdx.x, n = a.n;
   for (int w = wave; w < a.W; w += nw) {
     const int64_t row = (int64_t)b * a.W + w;
-    if (a.done && a.done[row]) continue;
+    const float score = a.scores[row];
+    // (the row is read whether its beam has ended or not: waiting for the flag
+    // would cost every row a trip to memory)
+    const bool ended = a.done && a.done[row];
     RowTop t;
-    if (FUSED) scan(a, row, 0, a.V, lane, t);
-    else join(a, row, lane, t);
-    if (lane < a.n) {
-      lv[w][lane] = t.v;
-      li[w][lane] = t.id;
+    if (FUSED) scan(a, row, 0, a.V, lane, buf[wave], t);
+    else join(a, row, lane, buf[wave], t);
+    if (ended) {  // as a row of one id, whose logarithm is 0
+      t.m = 0.f;
+      t.sum = 1.0;
+      t.v = lane == 0 ? 0.f : -INFINITY;
+      t.id = lane == 0 ? (uint32_t)a.end_id : kNoId;
+    }
+    if (lane < n) {
+      lv[w * n + lane] = t.v;
+      li[w * n + lane] = t.id;
     }
     if (lane == 0) {
       lm[w] = t.m;
-      ls[w] = t.sum;
+      ls[w] = log(t.sum);
+      sc[w] = (double)score;
     }
   }
   __syncthreads();
+  // c of every candidate, as a key (0: none)
+  const int all = a.W * n;
+  const uint32_t per = 65536 / n + 1;  // i / n as a product: i < 1024, n <= 32
+  for (int i = threadIdx.x; i < all; i += blockDim.x) {
+    const int w = (int)(i * per >> 16);
+    const float v = lv[i], m = lm[w];
+    const double c = sc[w] + ((v == m ? 0.0 : (double)v - (double)m) - ls[w]);
+    lk[i] = li[i] != kNoId && c > -INFINITY ? order_of(c) : 0ull;
+  }
+  __syncthreads();
   if (wave == 0) {
-    const bool mine = lane < a.W;
-    const double score = mine ? (double)a.scores[(int64_t)b * a.W + lane] : -INFINITY;
-    const bool ended = mine && a.done && a.done[(int64_t)b * a.W + lane];
-    const float m = mine && !ended ? lm[lane] : 0.f;
-    const double lsum = mine && !ended ? log(ls[lane]) : 0.0;
-    int at = 0;  // of the beam's list
-    auto head = [&](uint32_t& id) {
-      id = kNoId;
-      if (!mine || at >= a.n) return (double)-INFINITY;
-      if (ended) {
-        if (at) return (double)-INFINITY;
-        id = (uint32_t)a.end_id;
-        return score;
+    int mine;  // the candidate that lane k's output is
+    if (all <= 64) mine = best_of<1>(lk, all, n, lane, buf[0], at64);  // uniform
+    else if (all <= 128) mine = best_of<2>(lk, all, n, lane, buf[0], at64);
+    else if (all <= 256) mine = best_of<4>(lk, all, n, lane, buf[0], at64);
+    else mine = best_of<16>(lk, all, n, lane, buf[0], at64);
+    if (lane < n) {
+      const int64_t o = (int64_t)b * n + lane;
+      const int w = mine < 0 ? -1 : (int)(mine * per >> 16);
+      const int32_t id = mine < 0 ? -1 : (int32_t)li[mine];
+      float score = -INFINITY;
+      if (mine >= 0) {
+        const float v = lv[mine], m = lm[w];
+        score = (float)(sc[w] + ((v == m ? 0.0 : (double)v - (double)m) - ls[w]));
       }
-      id = li[lane][at];
-      if (id == kNoId) return (double)-INFINITY;
-      const float v = lv[lane][at];
-      return score + ((v == m ? 0.0 : (double)v - (double)m) - lsum);
-    };
-    uint32_t id;
-    double c = head(id);
-    for (int k = 0; k < a.n; k++) {
-      const uint64_t key = c > -INFINITY ? order_of(c) : 0ull;  // NaN: none
-      const uint32_t hi = wave_umax((uint32_t)(key >> 32));
-      const uint32_t lo = wave_umax((uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
-      const uint64_t who = __ballot(key && (uint32_t)(key >> 32) == hi && (uint32_t)key == lo);
-      const int w = who ? __ffsll((unsigned long long)who) - 1 : -1;  // the lowest beam on ties
-      const int64_t o = (int64_t)b * a.n + k;
-      if (w < 0 ? lane == 0 : lane == w) {
-        const int32_t id_out = w < 0 ? -1 : (int32_t)id;
-        a.scores_out[o] = w < 0 ? -INFINITY : (float)c;
-        a.parent[o] = w;
-        a.token[o] = id_out;
-        if (a.done_out) a.done_out[o] = w < 0 || (a.end_id >= 0 && id_out == a.end_id);
-        from[k] = w;
-        tok[k] = id_out;
-      }
-      if (lane == w) {
-        at++;
-        c = head(id);
-      }
+      a.scores_out[o] = score;
+      a.parent[o] = w;
+      a.token[o] = id;
+      if (a.done_out) a.done_out[o] = w < 0 || (a.end_id >= 0 && id == a.end_id);
+      from[lane] = w;
+      tok[lane] = id;
     }
   }
   if (!a.seen_out) return;
   __syncthreads();
   // every chosen beam's history: its parent's and the chosen id
-  for (int i = threadIdx.x; i < a.n * a.words; i += blockDim.x) {
-    const int k = i / a.words, j = i % a.words;
+  for (int k = wave; k < n; k += nw) {
     const int w = from[k], v = tok[k];
-    uint32_t bits = 0u;
-    if (w >= 0) {
-      bits = a.seen[((int64_t)b * a.W + w) * a.words + j];
-      if (v >> 5 == j) bits |= 1u << (v & 31);
+    const uint32_t* src = a.seen + ((int64_t)b * a.W + max(w, 0)) * a.words;
+    uint32_t* dst = a.seen_out + ((int64_t)b * n + k) * a.words;
+    for (int j = lane; j < a.words; j += 64) {
+      uint32_t bits = w >= 0 ? src[j] : 0u;
+      if (w >= 0 && v >> 5 == j) bits |= 1u << (v & 31);
+      dst[j] = bits;
     }
-    a.seen_out[((int64_t)b * a.n + k) * a.words + j] = bits;
   }
 }
 
@@ -398,7 +627,7 @@ struct ReorderIn {
 // and every byte is read where its parent still has it.  A group's slots are
 // cut into blockDim.x-thread pieces along blockIdx.y.
 template <int MW>
-__global__ __launch_bounds__(256) void k_ring_reorder(const ReorderIn a, int row_chunks) {
+__global__ __launch_bounds__(256) void k_ring_reorder(const ReorderIn a, int chunk_bits) {
   const int head = blockIdx.x % H;
   const int gl = blockIdx.x / H, group = gl % a.groups, layer = gl / a.groups;
   int64_t first = 0, n = a.C;
@@ -414,11 +643,13 @@ __global__ __launch_bounds__(256) void k_ring_reorder(const ReorderIn a, int row
     from[w] = p >= 0 && p < a.W && p != w ? p : -1;
   }
   const int64_t seq0 = (int64_t)layer * a.max_seqs + (int64_t)group * a.W;
-  const int64_t step = (int64_t)gridDim.y * 256;
-  for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < n * row_chunks; i += step) {
-    const int64_t slot = (first + i / row_chunks) % a.C;
-    const int piece = (int)(i % row_chunks);
-    const int64_t off = seq0 * a.seq_bytes + head * a.head_bytes + (slot * row_chunks + piece) * 16;
+  // (a row is 8 or 16 pieces, a head's run at most 2^28 bytes)
+  const uint32_t at0 = (uint32_t)first % (uint32_t)a.C, pieces = n > 0 ? (uint32_t)n << chunk_bits : 0u;
+  for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < pieces; i += gridDim.y * 256) {
+    uint32_t slot = at0 + (i >> chunk_bits);
+    if (slot >= (uint32_t)a.C) slot -= a.C;
+    const uint32_t piece = i & ((1u << chunk_bits) - 1);
+    const int64_t off = seq0 * a.seq_bytes + head * a.head_bytes + (((slot << chunk_bits) + piece) << 4);
     u32x4_t kk[MW], vv[MW];
 #pragma unroll
     for (int w = 0; w < MW; w++) {
@@ -466,14 +697,14 @@ int launch_ring_reorder(mb_ctx* ctx, int layer0, int n_layers, int B, int W, con
   a.parent = parent;
   a.from = from;
   a.to = to;
-  const int row_chunks = (int)(HD * e / 16);
+  const int chunk_bits = e == 2 ? 3 : 4, row_chunks = 1 << chunk_bits;  // 16-byte pieces of a row
   const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(max_rows, ring.C));
   const int64_t bx = (int64_t)n_layers * a.groups * H;
   const int64_t by = std::min<int64_t>(65535, (rows * row_chunks + 255) / 256);
   if (bx > INT32_MAX) return fail(ctx, MB_ERR_ARG, "too many rings in one call");
   const dim3 grid((unsigned)bx, (unsigned)by);
   auto go = [&](auto mw) {
-    hipLaunchKernelGGL(k_ring_reorder<decltype(mw)::value>, grid, dim3(256), 0, ctx->stream, a, row_chunks);
+    hipLaunchKernelGGL(k_ring_reorder<decltype(mw)::value>, grid, dim3(256), 0, ctx->stream, a, chunk_bits);
   };
   if (W <= 2) go(std::integral_constant<int, 2>{});
   else if (W <= 4) go(std::integral_constant<int, 4>{});

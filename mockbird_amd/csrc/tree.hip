@@ -41,7 +41,7 @@ struct TreeIn {
   float* out;
   int64_t out_stride;
   float* part;  // splits > 1: [unit][split][rows][PART]
-  int splits;
+  int splits, groups, units;
 };
 
 // Nodes of sequence b that are attended (0: none), and the first position.
@@ -69,18 +69,31 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t* parent, int n, int 
   return mask;
 }
 
-// Eight dims of a fused row as floats.
-__device__ __forceinline__ void load_row8(const TreeIn& a, int64_t off, float* x) {
-  if (a.qkv_bf16) load8<true>(a.qkv, off, x);
-  else load8<false>(a.qkv, off, x);
+// cos and sin of the four pairs from dim d0 on, all read at once; those of a
+// position beyond the table one after another (one copy of that code).
+__device__ __forceinline__ void rope4_cs(const float2* tab, int32_t pos, int d0, float2 (&t)[4]) {
+  const float4* r = (const float4*)(tab + (int64_t)min(pos, kRopeTab - 1) * 32 + (d0 >> 1));
+  const float4 u = r[0], v = r[1];
+  t[0] = make_float2(u.x, u.y);
+  t[1] = make_float2(u.z, u.w);
+  t[2] = make_float2(v.x, v.y);
+  t[3] = make_float2(v.z, v.w);
+  if (pos >= kRopeTab) {
+#pragma unroll 1
+    for (int j = 0; j < 4; j++) {
+      float c, s;
+      rope_cs(tab, pos, (d0 >> 1) + j, c, s);
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (j == k) t[k] = make_float2(c, s);
+    }
+  }
 }
-
-__device__ __forceinline__ void rope8(const float2* tab, int32_t pos, int d0, float* x) {
+__device__ __forceinline__ void rope8(const float2 (&t)[4], float* x) {
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    float c, s, a, b;
-    rope_cs(tab, pos, (d0 >> 1) + j, c, s);
-    rope_pair(x[2 * j], x[2 * j + 1], c, s, a, b);
+    float a, b;
+    rope_pair(x[2 * j], x[2 * j + 1], t[j].x, t[j].y, a, b);
     x[2 * j] = a;
     x[2 * j + 1] = b;
   }
@@ -137,16 +150,16 @@ struct TreeBatch {
 // The same rows again, for inputs that are not finite: lane = slot for the
 // scores, lane = dim for the sums.
 template <bool KV_BF16>
-__device__ __forceinline__ void exact_rows(const TreeIn& a, int b, int head, int split, int unit, int n,
-                                        int p0, uint64_t anc, const char* dk, const char* dv,
-                                        int dpitch) {
+__device__ __forceinline__ void exact_rows(const TreeIn& a, int b, int head, int split, int unit,
+                                           int node0, int n, int p0, uint64_t anc, const char* dk,
+                                           const char* dv, int dpitch) {
   constexpr int E = KV_BF16 ? 2 : 4, SB = KV_BF16 ? 32 : 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int nvalid = min(p0, a.C);
   const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
   const char *kb = a.k + off, *vb = a.v + off;
   const int32_t* sp = a.sp + (int64_t)b * a.C;
-  for (int node = wave; node < n; node += kTreeWaves) {
+  for (int node = node0 + wave; node < n; node += kTreeWaves) {
     const uint64_t mine = __shfl((uint64_t)anc, node);
     const int pos = p0 + __popcll(mine) - 1;
     const int64_t qoff = ((int64_t)b * a.rows + node) * a.row_stride + head * HD + lane;
@@ -200,14 +213,14 @@ __device__ __forceinline__ void exact_rows(const TreeIn& a, int b, int head, int
   }
 }
 
-template <bool KV_BF16, int NT>
-__global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
+template <bool KV_BF16, int NT, int G>
+__global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
   constexpr int SB = KV_BF16 ? 32 : 16;       // slots per batch
   constexpr int E = KV_BF16 ? 2 : 4;          // bytes per element
   constexpr int ROWB = HD * E;                // bytes per slot
   constexpr int NS = SB / 4;                  // slots of a batch per lane
   constexpr int NN = NT * 16;
-  constexpr int DR = (NN + SB - 1) / SB * SB; // drafted rows kept, in whole batches
+  constexpr int DR = (NN * G + SB - 1) / SB * SB; // drafted rows kept, in whole batches
   constexpr int QP = HD + 4;                  // floats per q row in LDS
   constexpr int DP = ROWB + 16;               // bytes per drafted row in LDS
   constexpr int FOLD = kTreeWaves * 16 * PART;
@@ -215,11 +228,17 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
   __shared__ __align__(16) char sdk[DR * DP], sdv[DR * DP];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int unit = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  // the G groups of one (sequence, head, split) are 8 workgroups apart
+  const int group = G == 1 ? 0 : blockIdx.x / 8 % G;
+  const int share = G == 1 ? blockIdx.x : blockIdx.x / (8 * G) * 8 + blockIdx.x % 8;
+  const int unit = share / a.splits, split = share % a.splits;
+  if (G > 1 && unit >= a.units) return;
   const int b = unit / H, head = unit % H;
   int p0;
   const int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
-  if (n <= 0) return;  // the whole workgroup
+  const int node0 = group * NN;  // this group's first node
+  if (n <= node0) return;        // the whole workgroup
+  const int tiles = min(NT, (n - node0 + 15) / 16);
   const int c = lane & 15, g = lane >> 4;
   const int nvalid = min(p0, a.C);
   const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
@@ -230,19 +249,19 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
   TreeBatch<KV_BF16> x;
   int32_t spl = -1;
   // Slots past the window read its last one (slot 0 of an empty window) and
-  // are dead by their position.
+  // are dead by their position.  (A head's run is at most 2^28 bytes.)
   const int last = max(nvalid - 1, 0);
   auto load_k = [&](int base) {
     spl = lane < SB && base + lane < nvalid ? sp[base + lane] : -1;
     if constexpr (KV_BF16) {
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const char* r = kb + (int64_t)min(base + 16 * u + c, last) * ROWB + g * 16;
+        const char* r = kb + (uint32_t)(min(base + 16 * u + c, last) * ROWB + g * 16);
 #pragma unroll
         for (int h = 0; h < 2; h++) x.k[2 * u + h] = __builtin_nontemporal_load((const u32x4_t*)(r + 64 * h));
       }
     } else {
-      const char* r = kb + (int64_t)min(base + c, last) * ROWB + g * 16;
+      const char* r = kb + (uint32_t)(min(base + c, last) * ROWB + g * 16);
 #pragma unroll
       for (int q = 0; q < 4; q++) x.k[q] = __builtin_nontemporal_load((const u32x4_t*)(r + 64 * q));
     }
@@ -250,7 +269,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
   auto load_v = [&](int base) {
 #pragma unroll
     for (int j = 0; j < NS; j++) {
-      const char* r = vb + (int64_t)min(base + 16 * (j >> 2) + 4 * g + (j & 3), last) * ROWB + c * 4 * E;
+      const char* r = vb + (uint32_t)(min(base + 16 * (j >> 2) + 4 * g + (j & 3), last) * ROWB + c * 4 * E);
       if constexpr (KV_BF16) x.v[j] = __builtin_nontemporal_load((const u32x2_t*)r);
       else x.v[j] = __builtin_nontemporal_load((const u32x4_t*)r);
     }
@@ -260,28 +279,37 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
 
   // the nodes' ancestors, and their q (and in the first split K and V) rows
   const uint64_t anc = ancestors(a.parent + (int64_t)b * a.rows, n, lane);
-  for (int i = threadIdx.x; i < DR * 8; i += 64 * kTreeWaves) {  // whole waves
+  const int keys = split == 0 ? min((n + SB - 1) / SB * SB, DR) : 0;  // drafted rows, in batches
+  const int rows0 = keys ? 0 : node0, rows = max(keys, node0 + NN);
+  for (int i = rows0 * 8 + threadIdx.x; i < rows * 8; i += 64 * kTreeWaves) {  // whole waves
     const int node = i >> 3, d0 = (i & 7) * 8, src = min(node, n - 1);
     const uint32_t lo = __shfl((uint32_t)anc, src), hi = __shfl((uint32_t)(anc >> 32), src);
     const int32_t pos = p0 + __popc(lo) + __popc(hi) - 1;
     const int64_t roff = ((int64_t)b * a.rows + src) * a.row_stride + head * HD + d0;
-    float r[8];
-    if (node < NN) {
-      load_row8(a, roff, r);
-      rope8(a.rope, pos, d0, r);
-#pragma unroll
-      for (int j = 0; j < 8; j++) sq[node * QP + d0 + j] = r[j] * 0.125f;  // exact
+    float r[8], k[8], v[8];
+    float2 cs[4];
+    if (a.qkv_bf16) {
+      load8<true>(a.qkv, roff, r);
+      load8<true>(a.qkv, roff + D, k);
+      load8<true>(a.qkv, roff + 2 * D, v);
+    } else {
+      load8<false>(a.qkv, roff, r);
+      load8<false>(a.qkv, roff + D, k);
+      load8<false>(a.qkv, roff + 2 * D, v);
     }
-    if (split == 0) {
-      load_row8(a, roff + D, r);
-      rope8(a.rope, pos, d0, r);
-      float w[8];
-      load_row8(a, roff + 2 * D, w);
+    rope4_cs(a.rope, pos, d0, cs);
+    if (node >= node0 && node < node0 + NN) {
+      rope8(cs, r);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sq[(node - node0) * QP + d0 + j] = r[j] * 0.125f;  // exact
+    }
+    if (node < keys) {
+      rope8(cs, k);
       if (node >= n)
 #pragma unroll
-        for (int j = 0; j < 8; j++) r[j] = w[j] = 0.f;
-      store8<KV_BF16>(sdk + node * DP, d0, r);
-      store8<KV_BF16>(sdv + node * DP, d0, w);
+        for (int j = 0; j < 8; j++) k[j] = v[j] = 0.f;
+      store8<KV_BF16>(sdk + node * DP, d0, k);
+      store8<KV_BF16>(sdv + node * DP, d0, v);
     }
   }
   // of the tiles' nodes c: position and ancestors
@@ -289,7 +317,8 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
   uint64_t sees[NT];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    const uint32_t lo = __shfl((uint32_t)anc, 16 * t + c), hi = __shfl((uint32_t)(anc >> 32), 16 * t + c);
+    const int node = node0 + 16 * t + c;
+    const uint32_t lo = __shfl((uint32_t)anc, node), hi = __shfl((uint32_t)(anc >> 32), node);
     sees[t] = (uint64_t)hi << 32 | lo;
     at[t] = p0 + __popcll(sees[t]) - 1;
   }
@@ -298,24 +327,41 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
   for (int o = 32; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o));
   __syncthreads();
 
-  // q as the second operand of the scores
-  std::conditional_t<KV_BF16, Planes[NT][2], f32x4_t[NT][4]> q;
+  // q as the second operand of the scores: in registers, or with two tiles of
+  // bf16 planes in LDS, in the lanes' order (48 registers less)
+  constexpr bool QLDS = KV_BF16 && NT > 1;
+  __shared__ uint4 sqp[QLDS ? NT * 2 : 1][3][QLDS ? 64 : 1];
+  std::conditional_t<KV_BF16, Planes[QLDS ? 1 : NT][2], f32x4_t[NT][4]> q;
+  auto planes = [&](int t, int h) {
+    const float* r = sq + (16 * t + c) * QP + 32 * h + 8 * g;
+    float v[8];
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const float* r = sq + (16 * t + c) * QP;
-    if constexpr (KV_BF16) {
+    for (int j = 0; j < 8; j++) v[j] = r[j];
+    return split3(v);
+  };
+  if constexpr (QLDS) {
+    for (int i = wave; i < NT * 2; i += kTreeWaves) {
+      const Planes p = planes(i >> 1, i & 1);
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        float v[8];
+      for (int k = 0; k < 3; k++) sqp[i][k][lane] = __builtin_bit_cast(uint4, p.p[k]);
+    }
+    __syncthreads();
+  } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = r[32 * h + 8 * g + j];
-        q[t][h] = split3(v);
+    for (int t = 0; t < NT; t++) {
+      if constexpr (KV_BF16) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) q[t][h] = planes(t, h);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) q[t][j] = *(const f32x4_t*)(sq + (16 * t + c) * QP + 16 * j + 4 * g);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++) q[t][j] = *(const f32x4_t*)(r + 16 * j + 4 * g);
     }
   }
+  auto plane = [&](auto& q, int t, int h, int k) {
+    if constexpr (QLDS) return __builtin_bit_cast(bf16x8_t, sqp[2 * t + h][k][lane]);
+    else return q[t][h].p[k];
+  };
 
   TreeState<KV_BF16, NT> st;
 #pragma unroll
@@ -330,27 +376,33 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
   float s[NT][NS];
   auto scores = [&]() {
 #pragma unroll
-    for (int t = 0; t < NT; t++)
+    for (int t = 0; t < NT; t++) {
+      if (NT > 1 && t >= tiles) break;  // uniform
+      if constexpr (KV_BF16) {
+        f32x4_t d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int u = 0; u < NS / 4; u++) {
+        for (int k = 2; k >= 0; k--)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const bf16x8_t p = plane(q, t, h, k);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+              d[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x.k[2 * u + h]), p,
+                                                             d[u], 0, 0, 0);
+          }
+#pragma unroll
+        for (int j = 0; j < 8; j++) s[t][j] = d[j >> 2][j & 3];
+      } else {
         f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (KV_BF16) {
 #pragma unroll
-          for (int p = 2; p >= 0; p--)
+        for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-              d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x.k[2 * u + h]),
-                                                          q[t][h].p[p], d, 0, 0, 0);
-        } else {
+          for (int e = 0; e < 4; e++)
+            d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[j][e]), q[t][j][e], d, 0, 0, 0);
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[j][e]), q[t][j][e], d, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[t][4 * u + i] = d[i];
+        for (int j = 0; j < 4; j++) s[t][j] = d[j];
       }
+    }
   };
   // the batch's scores into the states
   auto apply = [&]() {
@@ -368,6 +420,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
     }
 #pragma unroll
     for (int t = 0; t < NT; t++) {
+      if (NT > 1 && t >= tiles) break;
       float mx = s[t][0];
 #pragma unroll
       for (int j = 1; j < NS; j++) mx = fmaxf(mx, s[t][j]);
@@ -424,8 +477,8 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
     apply();
     if (more) load_v(base + step);
   }
-  if (split == 0) {
-    for (int base = wave * SB; base < DR; base += kTreeWaves * SB) {
+  {
+    for (int base = wave * SB; base < keys; base += kTreeWaves * SB) {
       if constexpr (KV_BF16) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -465,7 +518,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
       f[65] = l;
     }
     __syncthreads();
-    const int i = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, node = 16 * t + i;
+    const int i = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, node = node0 + 16 * t + i;
     float M = -INFINITY, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -495,44 +548,74 @@ __global__ __launch_bounds__(64 * kTreeWaves) void k_tree(const TreeIn a) {
     }
   }
   if (__syncthreads_or(bad))
-    exact_rows<KV_BF16>(a, b, head, split, unit, n, p0, anc, sdk, sdv, DP);
+    exact_rows<KV_BF16>(a, b, head, split, unit, node0, min(n, node0 + NN), p0, anc, sdk, sdv, DP);
 }
 
-// The states of a window shared by several workgroups: 16 nodes of one
-// (sequence, head) per workgroup.
+// The states of a window shared by several workgroups: a wave per node of one
+// (sequence, head), lane (g, quad) taking every fourth state's dims 4 quad ..
+// + 3, 16 states on their way at once.
 __global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a) {
   const int unit = blockIdx.x, b = unit / H, head = unit % H;
+  const int lane = threadIdx.x & 63, g = lane >> 4, d = (lane & 15) * 4;
   int p0;
   const int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
-  const int node = blockIdx.y * 16 + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
+  const int node = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (node >= n) return;
   const float* r = a.part + ((int64_t)unit * a.splits * a.rows + node) * PART;
   const int64_t step = (int64_t)a.rows * PART;
   float M = -INFINITY, L = 0.f;
-  for (int s = 0; s < a.splits; s++) M = fmaxf(M, r[s * step + 64]);
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; s++) {
-    const float m = r[s * step + 64], by = m == -INFINITY ? 0.f : __expf(m - M);
-    const f32x4_t v = *(const f32x4_t*)(r + s * step + d);
-    L += by * r[s * step + 65];
-    o += by * v;
+  for (int s0 = 0; s0 < a.splits; s0 += 16) {
+    f32x4_t v[4];
+    float m[4], l[4], mx = M;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float* p = r + min(s0 + 4 * j + g, a.splits - 1) * step;
+      v[j] = *(const f32x4_t*)(p + d);
+      m[j] = p[64];
+      l[j] = p[65];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (s0 + 4 * j + g >= a.splits) m[j] = -INFINITY;
+      mx = fmaxf(mx, m[j]);
+    }
+    const float by = M == -INFINITY ? 0.f : __expf(M - mx);
+    L *= by;
+    o *= by;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (m[j] != -INFINITY) {  // (a state that saw nothing may not be finite)
+        const float w = __expf(m[j] - mx);
+        L += w * l[j];
+        o += w * v[j];
+      }
+    M = mx;
   }
-  const float by = L == 0.f ? 0.f : 1.f / L;
-  *(f32x4_t*)(a.out + ((int64_t)b * a.rows + node) * a.out_stride + head * HD + d) = o * by;
+  // the four lane groups
+  const float mx = col_max(M), by = M == -INFINITY ? 0.f : __expf(M - mx);
+  L = col_sum(L * by);
+#pragma unroll
+  for (int i = 0; i < 4; i++) o[i] = col_sum(M == -INFINITY ? 0.f : o[i] * by);
+  if (g == 0) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *(f32x4_t*)(a.out + ((int64_t)b * a.rows + node) * a.out_stride + head * HD + d) = o * inv;
+  }
 }
 
 // Workgroups that share a (sequence, head)'s window: enough to fill the chip,
 // each wave with a batch of its own at least.
-static int tree_splits(const mb_ctx* ctx, int B, int32_t max_pos) {
-  const int64_t units = (int64_t)B * H, sb = ctx->cfg.kv_dtype == MB_KV_BF16 ? 32 : 16;
+static int tree_groups(int rows) { return rows <= 32 ? 1 : 2; }
+static int tree_splits(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
+  const int64_t units = (int64_t)B * H * tree_groups(rows), sb = ctx->cfg.kv_dtype == MB_KV_BF16 ? 32 : 16;
   const int64_t window = std::min<int64_t>(std::max(max_pos, 1), ctx->cfg.capacity);
-  const int64_t most = (window + sb * kTreeWaves - 1) / (sb * kTreeWaves);
+  const int64_t most = std::min<int64_t>(64, (window + sb * kTreeWaves - 1) / (sb * kTreeWaves));
   return (int)std::max<int64_t>(1, std::min(most, 768 / units));
 }
 
 int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
   if (B < 1) return 0;
-  const int s = tree_splits(ctx, B, max_pos);
+  const int s = tree_splits(ctx, B, rows, max_pos);
   return s > 1 ? (int64_t)B * H * s * rows * PART * 4 : 0;
 }
 
@@ -557,21 +640,25 @@ int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, co
   a.out = out;
   a.out_stride = out_stride;
   a.part = (float*)work;
-  a.splits = tree_splits(ctx, B, max_pos);
-  const dim3 grid((unsigned)(B * H * a.splits));
-  auto go = [&](auto nt) {
-    constexpr int NT = decltype(nt)::value;
-    if (ring.bf16) hipLaunchKernelGGL((k_tree<true, NT>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((k_tree<false, NT>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
+  a.splits = tree_splits(ctx, B, rows, max_pos);
+  a.groups = tree_groups(rows);
+  a.units = B * H;
+  const unsigned shares = (unsigned)(a.units * a.splits);
+  auto go = [&](auto nt, auto g) {
+    constexpr int NT = decltype(nt)::value, G = decltype(g)::value;
+    const dim3 grid(G == 1 ? shares : (shares + 7) / 8 * 8 * G);
+    if (ring.bf16) hipLaunchKernelGGL((k_tree<true, NT, G>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((k_tree<false, NT, G>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
   };
-  if (rows <= 16) go(std::integral_constant<int, 1>{});
-  else if (rows <= 32) go(std::integral_constant<int, 2>{});
-  else if (rows <= 48) go(std::integral_constant<int, 3>{});
-  else go(std::integral_constant<int, 4>{});
+  std::integral_constant<int, 1> one;
+  std::integral_constant<int, 2> two;
+  if (rows <= 16) go(one, one);
+  else if (rows <= 32) go(two, one);
+  else go(two, two);
   MB_HIP(ctx, hipGetLastError());
   if (a.splits > 1) {
-    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(B * H), (unsigned)((rows + 15) / 16)), dim3(256),
-                       0, ctx->stream, a);
+    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)a.units, (unsigned)((rows + 3) / 4)), dim3(256), 0,
+                       ctx->stream, a);
     MB_HIP(ctx, hipGetLastError());
   }
   return MB_OK;
@@ -588,45 +675,50 @@ template <bool IN_BF16, bool KV_BF16>
 __global__ __launch_bounds__(256) void k_tree_commit(
     const void* __restrict__ qkv, int64_t row_stride, int64_t layer_stride, int rows,
     const int32_t* __restrict__ pos0, const int32_t* __restrict__ path, int path_max,
-    const int32_t* __restrict__ n_path, int B, int n_layers, void* __restrict__ ring_k,
+    const int32_t* __restrict__ n_path, int B, void* __restrict__ ring_k,
     void* __restrict__ ring_v, int32_t* __restrict__ slot_pos, int64_t seq_stride,
     int64_t layer_seqs, int C, int wrap, const float2* __restrict__ rope_tab) {
-  const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t row_id = t / (H * 8);
-  if (row_id >= (int64_t)n_layers * B * path_max) return;
-  const int part = (int)(t % (H * 8)), head = part >> 3, d0 = (part & 7) * 8;
-  const int i = (int)(row_id % path_max);
-  const int b = (int)(row_id / path_max % B), layer = (int)(row_id / path_max / B);
-  const int n = min(n_path ? n_path[b] : path_max, path_max);
-  if (i >= n || (n > C && i < n - C)) return;
-  const int node = path[(int64_t)b * path_max + i];
-  const int64_t p64 = (int64_t)pos0[b] + i;
-  if (node < 0 || node >= rows || pos0[b] < 0 || p64 > INT32_MAX || (!wrap && p64 >= C)) return;
-  const int32_t pos = (int32_t)p64;
-  const int slot = wrap ? pos % C : pos;
-  const int64_t roff = layer * layer_stride + ((int64_t)b * rows + node) * row_stride + head * HD + d0;
-  float k[8], v[8];
-  load8<IN_BF16>(qkv, roff + D, k);
-  load8<IN_BF16>(qkv, roff + 2 * D, v);
-  rope8(rope_tab, pos, d0, k);
-  const int64_t seq = layer * layer_seqs + b;
-  const int64_t koff = seq * seq_stride + ((int64_t)head * C + slot) * HD + d0;
-  store8<KV_BF16>(ring_k, koff, k);
-  store8<KV_BF16>(ring_v, koff, v);
-  if (part == 0) slot_pos[seq * C + slot] = pos;
+  const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+  const int i = (int)(t / (H * 8)), part = (int)(t % (H * 8)), head = part >> 3, d0 = (part & 7) * 8;
+  if (i >= path_max) return;
+  const int layer = blockIdx.z;
+  for (int b = blockIdx.y; b < B; b += gridDim.y) {
+    // (the path's entry is read before its count is known: path_max bounds both)
+    const int n = min(n_path ? n_path[b] : path_max, path_max);
+    const int node = path[(int64_t)b * path_max + i];
+    const int32_t p0 = pos0[b];
+    const int64_t p64 = (int64_t)p0 + i;
+    if (i >= n || (n > C && i < n - C) || node < 0 || node >= rows || p0 < 0 || p64 > INT32_MAX ||
+        (!wrap && p64 >= C))
+      continue;
+    const int32_t pos = (int32_t)p64;
+    const int64_t roff = layer * layer_stride + ((int64_t)b * rows + node) * row_stride + head * HD + d0;
+    float k[8], v[8];
+    load8<IN_BF16>(qkv, roff + D, k);
+    load8<IN_BF16>(qkv, roff + 2 * D, v);
+    float2 cs[4];
+    rope4_cs(rope_tab, pos, d0, cs);
+    rope8(cs, k);
+    const int slot = wrap ? (int)((uint32_t)pos % (uint32_t)C) : pos;
+    const int64_t seq = layer * layer_seqs + b;
+    const int64_t koff = seq * seq_stride + ((int64_t)head * C + slot) * HD + d0;
+    store8<KV_BF16>(ring_k, koff, k);
+    store8<KV_BF16>(ring_v, koff, v);
+    if (part == 0) slot_pos[seq * C + slot] = pos;
+  }
 }
 
 int launch_tree_commit(mb_ctx* ctx, int layer0, int n_layers, int B, int rows, const void* qkv,
                        int qkv_dtype, int64_t qkv_stride, int64_t layer_stride, const int32_t* pos0,
                        int path_max, const int32_t* path, const int32_t* n_path) {
-  const int64_t threads = (int64_t)n_layers * B * path_max * H * 8;
-  const int64_t blocks = (threads + 255) / 256;
-  if (blocks > INT32_MAX) return fail(ctx, MB_ERR_ARG, "too many rows in one call");
+  const int64_t blocks = ((int64_t)path_max * H * 8 + 255) / 256;
+  if (blocks > INT32_MAX / 256) return fail(ctx, MB_ERR_ARG, "too many rows in one call");
   const RingView ring = global_ring(ctx, layer0);
+  const dim3 grid((unsigned)blocks, (unsigned)std::min(B, 65535), (unsigned)n_layers);
   auto go = [&](auto in, auto kv) {
-    hipLaunchKernelGGL((k_tree_commit<decltype(in)::value, decltype(kv)::value>), dim3((unsigned)blocks),
+    hipLaunchKernelGGL((k_tree_commit<decltype(in)::value, decltype(kv)::value>), grid,
                        dim3(256), 0, ctx->stream, qkv, qkv_stride, layer_stride, rows, pos0, path,
-                       path_max, n_path, B, n_layers, ring.k, ring.v, ring.sp, ring.seq_stride,
+                       path_max, n_path, B, ring.k, ring.v, ring.sp, ring.seq_stride,
                        (int64_t)ctx->cfg.max_seqs, ring.C, ring.wrap, ctx->rope_tab);
   };
   std::true_type yes;
