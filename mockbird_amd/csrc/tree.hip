@@ -40,8 +40,9 @@ struct TreeIn {
   const float2* rope;
   float* out;
   int64_t out_stride;
-  float* part;  // splits > 1: [unit][split][rows][PART]
-  int splits, groups, units;
+  int B, pieces;  // pieces 0: a workgroup per (sequence, head, group)
+  int32_t* plan;  // kPlanWords: the sequences' places on the line, and a piece's length
+  float* part;    // two states per workgroup and row
 };
 
 // Nodes of sequence b that are attended (0: none), and the first position.
@@ -52,12 +53,67 @@ __device__ __forceinline__ int tree_size(const int32_t* pos0, const int32_t* n_n
   return p0 < 0 || p0 > INT32_MAX - kTreeMaxNodes ? 0 : n;
 }
 
-// Lane i: the ancestors of node i, itself among them, one bit each.  Every
+// The work as a line.  A sequence's drafted rows are one quantum and every QS
+// slots of its window (a batch for each wave of a workgroup) another; the
+// sequences' quanta follow one another, and the line is cut into `pieces` equal
+// ones, one for each workgroup of a head (and group of nodes).  So all
+// workgroups have the same work whatever the windows' lengths are, and all fit
+// the chip at once.  (A workgroup for each sequence and head, or for each equal
+// share of a window, ended at 35 to 66 us over 24 windows of up to 1001 slots; more
+// and smaller workgroups than fit at once start under load, where each of their
+// three trips to memory takes several us.)
+// A state of a sequence that was cut goes to place 0 of its workgroup where the
+// sequence began before the piece, else to place 1.
+constexpr int kLineSeqs = 256, kPlanWords = 512;  // sequences on a line; words of TreeIn::plan
+template <int QS>
+__device__ __forceinline__ int quanta(const TreeIn& a, int b) {
+  int p0;
+  return tree_size(a.pos0, a.n_nodes, a.rows, b, p0) > 0 ? 1 + (min(p0, a.C) + QS - 1) / QS : 0;
+}
+// starts[i], i <= kLineSeqs: where sequence i begins (wave 0 writes them).  Every
+// lane returns the line's length and the sequence that holds quantum `at`
+// (undefined beyond the end), for the piece's own start and length.
+template <int QS>
+__device__ __forceinline__ int line(const TreeIn& a, int piece, int lane, bool write, int32_t* starts,
+                                    int& length, int& first) {
+  int q[4], sum = 0;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    q[k] = 4 * lane + k < a.B ? quanta<QS>(a, 4 * lane + k) : 0;
+    sum += q[k];
+  }
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(upto, o);
+    if (lane >= o) upto += t;
+  }
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+  length = max(1, (total + a.pieces - 1) / a.pieces);
+  const int at = piece * length;
+  int s = upto - sum, mine = 0;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    if (write) starts[4 * lane + k] = s;
+    if (at >= s && at < s + q[k]) mine = 4 * lane + k;
+    s += q[k];
+  }
+  if (write && lane == 63) starts[kLineSeqs] = total;
+  const uint64_t who = __ballot(at >= upto - sum && at < upto);
+  first = who ? __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)who) - 1) : 0;
+  return total;
+}
+// A workgroup's states of its place 0 or 1.
+__device__ __forceinline__ float* states(const TreeIn& a, int share, int group, int groups, int rows, int place) {
+  return a.part + (((int64_t)share * groups + group) * 2 + place) * rows * PART;
+}
+
+// Lane i, of parent `par`: the ancestors of node i, itself among them, one bit
+// each.  Every
 // round doubles the length of chain that a lane's mask covers.  A parent that
 // is not an earlier node counts as none.
-__device__ __forceinline__ uint64_t ancestors(const int32_t* parent, int n, int lane) {
-  int par = lane < n ? parent[lane] : -1;
-  if (par >= lane || par < 0) par = -1;
+__device__ __forceinline__ uint64_t ancestors(int32_t par, int n, int lane) {
+  if (lane >= n || par >= lane || par < 0) par = -1;
   uint64_t mask = 1ull << lane;
   while (__ballot(par >= 0)) {
     const int from = par >= 0 ? par : lane;
@@ -69,8 +125,40 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t* parent, int n, int 
   return mask;
 }
 
+// cos and sin of pair i at a position beyond the table: those of rope_cs, the
+// angle reduced by multiples of pi/2 (held in two doubles: the position's 31 bits
+// leave the remainder exact to 2^-53) and the Taylor series in double, its
+// coefficients read as it goes.  (The library's double functions, inlined in the
+// sequences' loop, keep some forty registers of constants through it.)
+__device__ const double kTrig[21] = {
+    // (-1)^n / (2n + 1)! and (-1)^n / (2n)!, n from 8 down
+    1.0 / 355687428096000.0, -1.0 / 1307674368000.0, 1.0 / 6227020800.0, -1.0 / 39916800.0, 1.0 / 362880.0,
+    -1.0 / 5040.0, 1.0 / 120.0, -1.0 / 6.0, 1.0,
+    1.0 / 20922789888000.0, -1.0 / 87178291200.0, 1.0 / 479001600.0, -1.0 / 3628800.0, 1.0 / 40320.0,
+    -1.0 / 720.0, 1.0 / 24.0, -1.0 / 2.0, 1.0,
+    // 2/pi, pi/2 and what pi/2 is above it
+    0x1.45f306dc9c883p-1, 0x1.921fb54442d18p+0, 0x1.1a62633145c07p-54};
+__device__ __forceinline__ float2 far_cs(int32_t pos, int i) {
+  const double a = (double)__fmul_rn((float)pos, __uint_as_float(c_inv_freq_bits[i]));
+  const double k = rint(a * kTrig[18]);
+  double r = fma(-k, kTrig[19], a);
+  r = fma(-k, kTrig[20], r);
+  const double r2 = r * r;
+  double sn = 0.0, cn = 0.0;
+#pragma unroll 1
+  for (int n = 0; n < 9; n++) {
+    sn = fma(sn, r2, kTrig[n]);
+    cn = fma(cn, r2, kTrig[9 + n]);
+  }
+  sn *= r;
+  const int q = (int)((int64_t)k & 3);
+  const double c = q & 1 ? sn : cn, s = q & 1 ? cn : sn;
+  return make_float2((float)(q == 1 || q == 2 ? -c : c), (float)(q >= 2 ? -s : s));
+}
+
 // cos and sin of the four pairs from dim d0 on, all read at once; those of a
 // position beyond the table one after another (one copy of that code).
+template <bool FAR_TAYLOR>
 __device__ __forceinline__ void rope4_cs(const float2* tab, int32_t pos, int d0, float2 (&t)[4]) {
   const float4* r = (const float4*)(tab + (int64_t)min(pos, kRopeTab - 1) * 32 + (d0 >> 1));
   const float4 u = r[0], v = r[1];
@@ -81,11 +169,12 @@ __device__ __forceinline__ void rope4_cs(const float2* tab, int32_t pos, int d0,
   if (pos >= kRopeTab) {
 #pragma unroll 1
     for (int j = 0; j < 4; j++) {
-      float c, s;
-      rope_cs(tab, pos, (d0 >> 1) + j, c, s);
+      float2 cs;
+      if constexpr (FAR_TAYLOR) cs = far_cs(pos, (d0 >> 1) + j);
+      else rope_cs(tab, pos, (d0 >> 1) + j, cs.x, cs.y);
 #pragma unroll
       for (int k = 0; k < 4; k++)
-        if (j == k) t[k] = make_float2(c, s);
+        if (j == k) t[k] = cs;
     }
   }
 }
@@ -99,13 +188,19 @@ __device__ __forceinline__ void rope8(const float2 (&t)[4], float* x) {
   }
 }
 
+// Part of a ring row, with the streaming hint where the launch reads it once.
+template <bool ONCE, class T>
+__device__ __forceinline__ T ring_load(const char* p) {
+  return ONCE ? __builtin_nontemporal_load((const T*)p) : *(const T*)p;
+}
+
 // One element of a K or V row.
 template <bool BF16>
 __device__ __forceinline__ float elem(const char* row, int d) {
   return BF16 ? bf16_lo(((const uint16_t*)row)[d]) : ((const float*)row)[d];
 }
 
-// One workgroup per (sequence, head, split).  A wave takes batches of SB slots
+// One workgroup per head and piece of the line (or sequence).  A wave takes batches of SB slots
 // (8 KB of K and V) in turn with the other waves of its (sequence, head),
 // forms the scores of all nodes, 16 to a tile, and keeps its own softmax state
 // per node; the waves' states are joined in LDS at the end, and those of
@@ -150,12 +245,11 @@ struct TreeBatch {
 // The same rows again, for inputs that are not finite: lane = slot for the
 // scores, lane = dim for the sums.
 template <bool KV_BF16>
-__device__ __forceinline__ void exact_rows(const TreeIn& a, int b, int head, int split, int unit,
-                                           int node0, int n, int p0, uint64_t anc, const char* dk,
-                                           const char* dv, int dpitch) {
-  constexpr int E = KV_BF16 ? 2 : 4, SB = KV_BF16 ? 32 : 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nvalid = min(p0, a.C);
+__device__ __forceinline__ void exact_rows(const TreeIn& a, int tid, int b, int head, int lo, int hi,
+                                           bool drafts, float* part, int node0, int n, int p0,
+                                           uint64_t anc, const char* dk, const char* dv, int dpitch) {
+  constexpr int E = KV_BF16 ? 2 : 4;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
   const char *kb = a.k + off, *vb = a.v + off;
   const int32_t* sp = a.sp + (int64_t)b * a.C;
@@ -165,9 +259,9 @@ __device__ __forceinline__ void exact_rows(const TreeIn& a, int b, int head, int
     const int64_t qoff = ((int64_t)b * a.rows + node) * a.row_stride + head * HD + lane;
     const float x = a.qkv_bf16 ? bf16_lo(((const uint16_t*)a.qkv)[qoff]) : ((const float*)a.qkv)[qoff];
     const float y = __shfl_xor(x, 1);
-    float c, s, r0, r1;
-    rope_cs(a.rope, pos, lane >> 1, c, s);
-    rope_pair(lane & 1 ? y : x, lane & 1 ? x : y, c, s, r0, r1);
+    float r0, r1;
+    const float2 cs = pos < kRopeTab ? a.rope[(int64_t)pos * 32 + (lane >> 1)] : far_cs(pos, lane >> 1);
+    rope_pair(lane & 1 ? y : x, lane & 1 ? x : y, cs.x, cs.y, r0, r1);
     const float q = (lane & 1 ? r1 : r0) * 0.125f;
     float m = -INFINITY, l = 0.f, acc = 0.f;
     auto rows = [&](const char* kr, const char* vr, int64_t pitch, bool live) {
@@ -190,18 +284,15 @@ __device__ __forceinline__ void exact_rows(const TreeIn& a, int b, int head, int
         if ((who >> j) & 1) acc = fmaf(wj, elem<KV_BF16>(vr + j * pitch, lane), acc);
       }
     };
-    for (int base = split * kTreeWaves * SB; base < nvalid; base += a.splits * kTreeWaves * SB)
-      for (int w0 = 0; w0 < kTreeWaves * SB; w0 += SB) {
-        const int slot = base + w0 + lane;
-        const int p = lane < SB && slot < nvalid ? sp[slot] : -1;
-        const bool live = p >= 0 && p < p0 && (int64_t)pos - p < a.C;
-        if (__ballot(live))
-          rows(kb + (int64_t)(base + w0) * HD * E, vb + (int64_t)(base + w0) * HD * E, HD * E, live);
-      }
-    if (split == 0) rows(dk, dv, dpitch, lane < n && ((mine >> lane) & 1));
+    for (int base = lo; base < hi; base += 64) {
+      const int p = base + lane < hi ? sp[base + lane] : -1;
+      const bool live = p >= 0 && p < p0 && (int64_t)pos - p < a.C;
+      if (__ballot(live)) rows(kb + (int64_t)base * HD * E, vb + (int64_t)base * HD * E, HD * E, live);
+    }
+    if (drafts) rows(dk, dv, dpitch, lane < n && ((mine >> lane) & 1));
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-    if (a.splits > 1) {
-      float* pp = a.part + (((int64_t)unit * a.splits + split) * a.rows + node) * PART;
+    if (part) {
+      float* pp = part + (node - node0) * PART;
       pp[lane] = acc;
       if (lane == 0) {
         pp[64] = m;
@@ -227,104 +318,156 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
   __shared__ __align__(16) float sq[NN * QP > FOLD ? NN * QP : FOLD];
   __shared__ __align__(16) char sdk[DR * DP], sdv[DR * DP];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // the G groups of one (sequence, head, split) are 8 workgroups apart
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the G groups of one piece are 8 workgroups apart: on one XCD, reading alike
+  constexpr int QS = kTreeWaves * SB;
   const int group = G == 1 ? 0 : blockIdx.x / 8 % G;
   const int share = G == 1 ? blockIdx.x : blockIdx.x / (8 * G) * 8 + blockIdx.x % 8;
-  const int unit = share / a.splits, split = share % a.splits;
-  if (G > 1 && unit >= a.units) return;
-  const int b = unit / H, head = unit % H;
-  int p0;
-  const int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
+  const int piece = share / H, head = share % H;
   const int node0 = group * NN;  // this group's first node
-  if (n <= node0) return;        // the whole workgroup
-  const int tiles = min(NT, (n - node0 + 15) / 16);
-  const int c = lane & 15, g = lane >> 4;
+  __shared__ int32_t starts[kLineSeqs + 1], flag[kTreeWaves];
+  int first = piece, end = a.B, from = 0, to = 0;  // the piece: quanta [from, to) from sequence `first` on
+  if (a.pieces) {
+    if (G > 1 && piece >= a.pieces) return;
+    int length;
+    const int total = line<QS>(a, piece, lane, wave == 0, starts, length, first);
+    __syncthreads();
+    if (blockIdx.x == 0) {  // for the merge
+      for (int i = threadIdx.x; i <= kLineSeqs; i += 64 * kTreeWaves) a.plan[i] = starts[i];
+      if (threadIdx.x == 0) a.plan[kLineSeqs + 1] = length;
+    }
+    from = piece * length;
+    to = min(total, from + length);
+    if (from >= to) return;
+  } else {
+    if (G > 1 && piece >= a.B) return;
+    end = piece + 1;
+  }
+
+  for (int b = first; b < end; b++) {
+  // (the thread's places are worked out anew for each sequence: kept over the
+  // loop they would take more registers than there are)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int32_t par = a.parent[(int64_t)b * a.rows + min(lane, a.rows - 1)];
+  int p0;
+  int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
+  n = __builtin_amdgcn_readfirstlane(n);
+  p0 = __builtin_amdgcn_readfirstlane(p0);
   const int nvalid = min(p0, a.C);
+  int lo = 0, hi = nvalid;  // this workgroup's slots of the window
+  bool drafts = true;       // and whether it has the drafted rows
+  float* part = nullptr;    // where its states go; null: it has the whole sequence
+  if (a.pieces) {
+    const int s0 = __builtin_amdgcn_readfirstlane(starts[b]), s1 = __builtin_amdgcn_readfirstlane(starts[b + 1]);
+    if (s0 >= to) break;
+    if (s0 == s1) continue;
+    const int j0 = max(from - s0, 0), j1 = min(to, s1) - s0;
+    drafts = j0 == 0;
+    lo = max(j0 - 1, 0) * QS;
+    hi = min(nvalid, (j1 - 1) * QS);
+    if (s0 < from || s1 > to) part = states(a, share, group, G, min(a.rows, NN), s0 < from ? 0 : 1);
+  }
+  if (n <= node0) continue;
+  const int tiles = min(NT, (n - node0 + 15) / 16);
   const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
   const char *kb = a.k + off, *vb = a.v + off;
   const int32_t* sp = a.sp + (int64_t)b * a.C;
-  const int s0 = (split * kTreeWaves + wave) * SB, step = a.splits * kTreeWaves * SB;
+
+  // The nodes' rows: q of this group's, and with the drafted rows K and V of every
+  // node that they may descend from; 32 rows at a time, thread -> row i / 8, dims
+  // 8 (i % 8) on.  Loads return in the order they are issued, so these go before
+  // the window's.
+  const int keys = drafts ? min((min(n, node0 + NN) + SB - 1) / SB * SB, DR) : 0;  // in batches
+  int row0 = keys ? 0 : node0;
+  const int d0 = (tid & 7) * 8;
+  const uint64_t anc = ancestors(par, n, lane);
+  float rq[8], rk[8], rv[8];
+  float2 cs[4];
+  auto load_rows = [&]() {
+    const int src = min(row0 + (tid >> 3), n - 1);
+    const int64_t roff = ((int64_t)b * a.rows + src) * a.row_stride + head * HD + d0;
+    if (a.qkv_bf16) {
+      load8<true>(a.qkv, roff, rq);
+      load8<true>(a.qkv, roff + D, rk);
+      load8<true>(a.qkv, roff + 2 * D, rv);
+    } else {
+      load8<false>(a.qkv, roff, rq);
+      load8<false>(a.qkv, roff + D, rk);
+      load8<false>(a.qkv, roff + 2 * D, rv);
+    }
+    const uint32_t al = __shfl((uint32_t)anc, src), ah = __shfl((uint32_t)(anc >> 32), src);
+    rope4_cs<true>(a.rope, p0 + __popc(al) + __popc(ah) - 1, d0, cs);
+  };
+  auto store_rows = [&]() {
+    const int node = row0 + (tid >> 3);
+    if (node >= node0 && node < node0 + NN) {
+      rope8(cs, rq);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sq[(node - node0) * QP + d0 + j] = rq[j] * 0.125f;  // exact
+    }
+    if (node < keys) {
+      rope8(cs, rk);
+      if (node >= n)
+#pragma unroll
+        for (int j = 0; j < 8; j++) rk[j] = rv[j] = 0.f;
+      store8<KV_BF16>(sdk + node * DP, d0, rk);
+      store8<KV_BF16>(sdv + node * DP, d0, rv);
+    }
+  };
+  static_assert(NN <= 8 * kTreeWaves, "a group's rows are read at once");
+  if (G > 1 && row0 < node0) {  // the second group's keys begin with the first's rows
+    load_rows();
+    store_rows();
+    row0 = node0;
+  }
+  load_rows();
+  __builtin_amdgcn_sched_barrier(0);
 
   TreeBatch<KV_BF16> x;
-  int32_t spl = -1;
+  int32_t spl;  // lane l: the stored position of the batch's slot l % SB
   // Slots past the window read its last one (slot 0 of an empty window) and
   // are dead by their position.  (A head's run is at most 2^28 bytes.)
-  const int last = max(nvalid - 1, 0);
+  const int last = max(hi - 1, 0);
   auto load_k = [&](int base) {
-    spl = lane < SB && base + lane < nvalid ? sp[base + lane] : -1;
+    spl = sp[min(base + (lane & (SB - 1)), last)];
     if constexpr (KV_BF16) {
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const char* r = kb + (uint32_t)(min(base + 16 * u + c, last) * ROWB + g * 16);
 #pragma unroll
-        for (int h = 0; h < 2; h++) x.k[2 * u + h] = __builtin_nontemporal_load((const u32x4_t*)(r + 64 * h));
+        for (int h = 0; h < 2; h++) x.k[2 * u + h] = ring_load<G == 1, u32x4_t>(r + 64 * h);
       }
     } else {
       const char* r = kb + (uint32_t)(min(base + c, last) * ROWB + g * 16);
 #pragma unroll
-      for (int q = 0; q < 4; q++) x.k[q] = __builtin_nontemporal_load((const u32x4_t*)(r + 64 * q));
+      for (int q = 0; q < 4; q++) x.k[q] = ring_load<G == 1, u32x4_t>(r + 64 * q);
     }
   };
   auto load_v = [&](int base) {
 #pragma unroll
     for (int j = 0; j < NS; j++) {
       const char* r = vb + (uint32_t)(min(base + 16 * (j >> 2) + 4 * g + (j & 3), last) * ROWB + c * 4 * E);
-      if constexpr (KV_BF16) x.v[j] = __builtin_nontemporal_load((const u32x2_t*)r);
-      else x.v[j] = __builtin_nontemporal_load((const u32x4_t*)r);
+      if constexpr (KV_BF16) x.v[j] = ring_load<G == 1, u32x2_t>(r);
+      else x.v[j] = ring_load<G == 1, u32x4_t>(r);
     }
   };
+  const int s0 = lo + wave * SB, step = kTreeWaves * SB;
   load_k(s0);
   load_v(s0);
+  __builtin_amdgcn_sched_barrier(0);
 
-  // the nodes' ancestors, and their q (and in the first split K and V) rows
-  const uint64_t anc = ancestors(a.parent + (int64_t)b * a.rows, n, lane);
-  const int keys = split == 0 ? min((n + SB - 1) / SB * SB, DR) : 0;  // drafted rows, in batches
-  const int rows0 = keys ? 0 : node0, rows = max(keys, node0 + NN);
-  for (int i = rows0 * 8 + threadIdx.x; i < rows * 8; i += 64 * kTreeWaves) {  // whole waves
-    const int node = i >> 3, d0 = (i & 7) * 8, src = min(node, n - 1);
-    const uint32_t lo = __shfl((uint32_t)anc, src), hi = __shfl((uint32_t)(anc >> 32), src);
-    const int32_t pos = p0 + __popc(lo) + __popc(hi) - 1;
-    const int64_t roff = ((int64_t)b * a.rows + src) * a.row_stride + head * HD + d0;
-    float r[8], k[8], v[8];
-    float2 cs[4];
-    if (a.qkv_bf16) {
-      load8<true>(a.qkv, roff, r);
-      load8<true>(a.qkv, roff + D, k);
-      load8<true>(a.qkv, roff + 2 * D, v);
-    } else {
-      load8<false>(a.qkv, roff, r);
-      load8<false>(a.qkv, roff + D, k);
-      load8<false>(a.qkv, roff + 2 * D, v);
-    }
-    rope4_cs(a.rope, pos, d0, cs);
-    if (node >= node0 && node < node0 + NN) {
-      rope8(cs, r);
-#pragma unroll
-      for (int j = 0; j < 8; j++) sq[(node - node0) * QP + d0 + j] = r[j] * 0.125f;  // exact
-    }
-    if (node < keys) {
-      rope8(cs, k);
-      if (node >= n)
-#pragma unroll
-        for (int j = 0; j < 8; j++) k[j] = v[j] = 0.f;
-      store8<KV_BF16>(sdk + node * DP, d0, k);
-      store8<KV_BF16>(sdv + node * DP, d0, v);
-    }
-  }
-  // of the tiles' nodes c: position and ancestors
-  int32_t at[NT];
-  uint64_t sees[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
+  store_rows();
+  auto ancestors_of = [&](int t) {
     const int node = node0 + 16 * t + c;
-    const uint32_t lo = __shfl((uint32_t)anc, node), hi = __shfl((uint32_t)(anc >> 32), node);
-    sees[t] = (uint64_t)hi << 32 | lo;
-    at[t] = p0 + __popcll(sees[t]) - 1;
-  }
+    const uint32_t al = __shfl((uint32_t)anc, node), ah = __shfl((uint32_t)(anc >> 32), node);
+    return (uint64_t)ah << 32 | al;
+  };
   int deepest = lane < n ? __popcll(anc) - 1 : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o));
+  deepest = __builtin_amdgcn_readfirstlane(deepest);
   __syncthreads();
 
   // q as the second operand of the scores: in registers, or with two tiles of
@@ -457,25 +600,26 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
     }
   };
 
-  for (int base = s0; base < nvalid; base += step) {
-    const int32_t sc = spl;
-    const bool more = base + step < nvalid;
+  for (int base = s0; base < hi; base += step) {
+    const int32_t sc = base + (lane & (SB - 1)) < hi ? spl : -1;
     scores();
-    if (more) load_k(base + step);
-    const uint64_t all = __ballot(sc >= 0 && sc < p0 && p0 + deepest - sc < a.C);
-    constexpr uint64_t full = (1ull << SB) - 1;
-    if (all != full) {  // uniform
+    // (loaded past the last batch too, from the last slot: a branch around the
+    // loads would have the next wait drain them all)
+    load_k(base + step);
+    const uint64_t all = __ballot((sc >= 0) & (sc < p0) & (p0 + deepest - sc < a.C));
+    if (~all) {  // uniform
 #pragma unroll
-      for (int j = 0; j < NS; j++) {
-        const int32_t p = __shfl(sc, 16 * (j >> 2) + 4 * g + (j & 3));
-        const bool cached = p >= 0 && p < p0;
+      for (int t = 0; t < NT; t++) {
+        const int32_t at = p0 + __popcll(ancestors_of(t)) - 1;
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-          if (!(cached && at[t] - p < a.C)) s[t][j] = -INFINITY;
+        for (int j = 0; j < NS; j++) {
+          const int32_t p = __shfl(sc, 16 * (j >> 2) + 4 * g + (j & 3));
+          s[t][j] = ((p >= 0) & (p < p0) & (at - p < a.C)) ? s[t][j] : -INFINITY;
+        }
       }
     }
     apply();
-    if (more) load_v(base + step);
+    load_v(base + step);
   }
   {
     for (int base = wave * SB; base < keys; base += kTreeWaves * SB) {
@@ -493,12 +637,14 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
             sdv + (base + 16 * (j >> 2) + 4 * g + (j & 3)) * DP + c * 4 * E);
       scores();
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+      for (int t = 0; t < NT; t++) {
+        const uint64_t sees = ancestors_of(t);
 #pragma unroll
         for (int j = 0; j < NS; j++) {
           const int row = base + 16 * (j >> 2) + 4 * g + (j & 3);
-          if (!((sees[t] >> row) & 1)) s[t][j] = -INFINITY;
+          if (!((sees >> row) & 1)) s[t][j] = -INFINITY;
         }
+      }
       apply();
     }
   }
@@ -518,7 +664,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
       f[65] = l;
     }
     __syncthreads();
-    const int i = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, node = node0 + 16 * t + i;
+    const int i = tid >> 4, d = (tid & 15) * 4, node = node0 + 16 * t + i;
     float M = -INFINITY, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -533,8 +679,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
     if (node < n) {
       bad |= !(fabsf(o[0]) < INFINITY && fabsf(o[1]) < INFINITY && fabsf(o[2]) < INFINITY &&
                fabsf(o[3]) < INFINITY && fabsf(L) < INFINITY && M < INFINITY);
-      if (a.splits > 1) {
-        float* pp = a.part + (((int64_t)unit * a.splits + split) * a.rows + node) * PART;
+      if (part) {
+        float* pp = part + (node - node0) * PART;
         *(f32x4_t*)(pp + d) = o;
         if (d == 0) {
           pp[64] = M;
@@ -547,37 +693,50 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
       }
     }
   }
-  if (__syncthreads_or(bad))
-    exact_rows<KV_BF16>(a, b, head, split, unit, node0, min(n, node0 + NN), p0, anc, sdk, sdv, DP);
+  const bool any = __ballot(bad) != 0;
+  if (lane == 0) flag[wave] = any;
+  __syncthreads();
+  static_assert(kTreeWaves == 4, "four flags");
+  if (flag[0] | flag[1] | flag[2] | flag[3]) {
+    exact_rows<KV_BF16>(a, tid, b, head, lo, hi, drafts, part, node0, min(n, node0 + NN), p0, anc, sdk, sdv, DP);
+    __syncthreads();
+  }
+  }
 }
 
-// The states of a window shared by several workgroups: a wave per node of one
-// (sequence, head), lane (g, quad) taking every fourth state's dims 4 quad ..
-// + 3, 16 states on their way at once.
-__global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a) {
-  const int unit = blockIdx.x, b = unit / H, head = unit % H;
+// The states of a sequence that was cut: a wave per node of one (sequence,
+// head), lane (g, quad) taking every fourth state's dims 4 quad .. + 3, 16 states
+// on their way at once.
+__global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a, int groups) {
+  const int b = blockIdx.x / H, head = blockIdx.x % H;
   const int lane = threadIdx.x & 63, g = lane >> 4, d = (lane & 15) * 4;
+  const int s = a.plan[b], e = a.plan[b + 1], length = a.plan[kLineSeqs + 1];
   int p0;
   const int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
   const int node = blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (node >= n) return;
-  const float* r = a.part + ((int64_t)unit * a.splits * a.rows + node) * PART;
-  const int64_t step = (int64_t)a.rows * PART;
+  if (node >= n || e == s) return;
+  const int first = s / length, splits = (e - 1) / length - first + 1;
+  if (splits == 1) return;
+  const int rows = min(a.rows, 32), group = node / 32;
+  // the first piece's place 1, the others' place 0
+  auto state = [&](int i) {
+    return states(a, (first + i) * H + head, group, groups, rows, i == 0) + (node - 32 * group) * PART;
+  };
   float M = -INFINITY, L = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < a.splits; s0 += 16) {
+  for (int s0 = 0; s0 < splits; s0 += 16) {
     f32x4_t v[4];
     float m[4], l[4], mx = M;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const float* p = r + min(s0 + 4 * j + g, a.splits - 1) * step;
+      const float* p = state(min(s0 + 4 * j + g, splits - 1));
       v[j] = *(const f32x4_t*)(p + d);
       m[j] = p[64];
       l[j] = p[65];
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      if (s0 + 4 * j + g >= a.splits) m[j] = -INFINITY;
+      if (s0 + 4 * j + g >= splits) m[j] = -INFINITY;
       mx = fmaxf(mx, m[j]);
     }
     const float by = M == -INFINITY ? 0.f : __expf(M - mx);
@@ -603,20 +762,20 @@ __global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a) {
   }
 }
 
-// Workgroups that share a (sequence, head)'s window: enough to fill the chip,
-// each wave with a batch of its own at least.
+// Workgroups per head of a launch whose work is cut as a line: with the groups
+// and heads as many as fit the chip at once (three per CU).  0: as many sequences
+// as fill the chip by themselves.
 static int tree_groups(int rows) { return rows <= 32 ? 1 : 2; }
-static int tree_splits(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
-  const int64_t units = (int64_t)B * H * tree_groups(rows), sb = ctx->cfg.kv_dtype == MB_KV_BF16 ? 32 : 16;
-  const int64_t window = std::min<int64_t>(std::max(max_pos, 1), ctx->cfg.capacity);
-  const int64_t most = std::min<int64_t>(64, (window + sb * kTreeWaves - 1) / (sb * kTreeWaves));
-  return (int)std::max<int64_t>(1, std::min(most, 768 / units));
+static int tree_pieces(const mb_ctx* ctx, int B, int rows) {
+  const int cus = ctx->cus_per_xcd > 0 ? ctx->xcds * ctx->cus_per_xcd : 256;
+  const int pieces = std::max(1, 3 * cus / (H * tree_groups(rows)));
+  return B < pieces && B <= kLineSeqs ? pieces : 0;
 }
 
-int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
+int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t) {
   if (B < 1) return 0;
-  const int s = tree_splits(ctx, B, rows, max_pos);
-  return s > 1 ? (int64_t)B * H * s * rows * PART * 4 : 0;
+  const int64_t g = tree_groups(rows), p = tree_pieces(ctx, B, rows);
+  return p ? 4 * (kPlanWords + p * H * g * 2 * std::min(rows, 32) * PART) : 0;
 }
 
 int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, const void* qkv,
@@ -639,11 +798,12 @@ int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, co
   a.rope = ctx->rope_tab;
   a.out = out;
   a.out_stride = out_stride;
-  a.part = (float*)work;
-  a.splits = tree_splits(ctx, B, rows, max_pos);
-  a.groups = tree_groups(rows);
-  a.units = B * H;
-  const unsigned shares = (unsigned)(a.units * a.splits);
+  a.B = B;
+  a.pieces = tree_pieces(ctx, B, rows);
+  a.plan = (int32_t*)work;
+  a.part = (float*)work + kPlanWords;
+  const int groups = tree_groups(rows);
+  const unsigned shares = (unsigned)((a.pieces ? a.pieces : B) * H);
   auto go = [&](auto nt, auto g) {
     constexpr int NT = decltype(nt)::value, G = decltype(g)::value;
     const dim3 grid(G == 1 ? shares : (shares + 7) / 8 * 8 * G);
@@ -656,9 +816,9 @@ int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, co
   else if (rows <= 32) go(two, one);
   else go(two, two);
   MB_HIP(ctx, hipGetLastError());
-  if (a.splits > 1) {
-    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)a.units, (unsigned)((rows + 3) / 4)), dim3(256), 0,
-                       ctx->stream, a);
+  if (a.pieces) {
+    hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(B * H), (unsigned)((rows + 3) / 4)), dim3(256), 0,
+                       ctx->stream, a, groups);
     MB_HIP(ctx, hipGetLastError());
   }
   return MB_OK;
@@ -697,7 +857,7 @@ __global__ __launch_bounds__(256) void k_tree_commit(
     load8<IN_BF16>(qkv, roff + D, k);
     load8<IN_BF16>(qkv, roff + 2 * D, v);
     float2 cs[4];
-    rope4_cs(rope_tab, pos, d0, cs);
+    rope4_cs<false>(rope_tab, pos, d0, cs);
     rope8(cs, k);
     const int slot = wrap ? (int)((uint32_t)pos % (uint32_t)C) : pos;
     const int64_t seq = layer * layer_seqs + b;
