@@ -370,14 +370,10 @@ __global__ __launch_bounds__(256) void k_beam_scan(const BeamIn a, int64_t parts
   if (lane < a.n) ((uint2*)(p + sizeof(PartRow)))[lane] = make_uint2(__float_as_uint(t.v), t.id);
 }
 
-// The parts of a row joined.
+// The parts of a row joined.  Everything is read before anything is used.
 __device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, uint64_t* buf, RowTop& t) {
   PartRow h{0.0, -INFINITY, 0u};
   if (lane < a.chunks) h = *(const PartRow*)part_row(a, row, lane);
-  t.m = wave_max(h.m);
-  // (an infinite maximum is the maximum of a part only where it was reached)
-  const double by = h.m == t.m ? 1.0 : (double)__expf(h.m - t.m);
-  t.sum = wave_sum(h.sum * by);
   const int all = a.chunks * a.n;
   const uint32_t per = (1u << 20) / a.n + 1;  // i / n as a product: i < 2^11, n <= 2^5
   for (int base = 0; base < all; base += kScan) {
@@ -396,6 +392,10 @@ __device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, uin
     }
     take_top(z, [&](int j) { return ids[j]; }, a.n, lane, buf, t);
   }
+  t.m = wave_max(h.m);
+  // (an infinite maximum is the maximum of a part only where it was reached)
+  const double by = h.m == t.m ? 1.0 : (double)__expf(h.m - t.m);
+  t.sum = wave_sum(h.sum * by);
 }
 
 // The n best of `all` <= 64 J keys in LDS, the lower index first on equal ones,

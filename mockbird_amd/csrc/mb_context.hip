@@ -194,6 +194,24 @@ int check_common(mb_ctx* ctx, int layer, int B) {
   return MB_OK;
 }
 
+// (cos, sin) of float(pos) * inv_freq[i], in double, rounded to fp32; made once
+// per process (some 25 ms), for every context.
+const std::vector<float2>& rope_table() {
+  static const std::vector<float2> table = [] {
+    std::vector<float2> tab((size_t)kRopeTab * 32);
+    for (int i = 0; i < 32; i++) {
+      float inv;
+      memcpy(&inv, &kInvFreqBits[i], 4);
+      for (int p = 0; p < kRopeTab; p++) {
+        const float a = (float)p * inv;
+        tab[(size_t)p * 32 + i] = make_float2((float)cos((double)a), (float)sin((double)a));
+      }
+    }
+    return tab;
+  }();
+  return table;
+}
+
 int check_layers(mb_ctx* ctx, int layer0, int n_layers, int B) {
   const int rc = check_common(ctx, layer0, B);
   if (rc) return rc;
@@ -303,16 +321,7 @@ int mb_create(const mb_config* cfg, mb_ctx** out) {
     e = hipMalloc(&ctx->slot_pos, (size_t)slots * sizeof(int32_t));
     if (e != hipSuccess) { rc = hip_fail(ctx, e, "hipMalloc(slot_pos)"); break; }
     {
-      // (cos, sin) of float(pos) * inv_freq[i], in double, rounded to fp32
-      std::vector<float2> tab((size_t)kRopeTab * 32);
-      for (int i = 0; i < 32; i++) {
-        float inv;
-        memcpy(&inv, &kInvFreqBits[i], 4);
-        for (int p = 0; p < kRopeTab; p++) {
-          const float a = (float)p * inv;
-          tab[(size_t)p * 32 + i] = make_float2((float)cos((double)a), (float)sin((double)a));
-        }
-      }
+      const std::vector<float2>& tab = rope_table();
       e = hipMalloc(&ctx->rope_tab, tab.size() * sizeof(float2));
       if (e != hipSuccess) { rc = hip_fail(ctx, e, "hipMalloc(rope table)"); break; }
       e = hipMemcpy(ctx->rope_tab, tab.data(), tab.size() * sizeof(float2), hipMemcpyHostToDevice);

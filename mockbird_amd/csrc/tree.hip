@@ -64,43 +64,41 @@ __device__ __forceinline__ int tree_size(const int32_t* pos0, const int32_t* n_n
 // three trips to memory takes several us.)
 // A state of a sequence that was cut goes to place 0 of its workgroup where the
 // sequence began before the piece, else to place 1.
-constexpr int kLineSeqs = 256, kPlanWords = 512;  // sequences on a line; words of TreeIn::plan
-template <int QS>
-__device__ __forceinline__ int quanta(const TreeIn& a, int b) {
-  int p0;
-  return tree_size(a.pos0, a.n_nodes, a.rows, b, p0) > 0 ? 1 + (min(p0, a.C) + QS - 1) / QS : 0;
+constexpr int kLineSeqs = 64, kPlanWords = 192;  // sequences on a line; words of TreeIn::plan
+// The line's places in LDS: where sequence i begins (starts[kLineSeqs]: the end),
+// its position and its nodes.
+struct Line {
+  int32_t starts[kLineSeqs + 1], p0[kLineSeqs], n[kLineSeqs];
+};
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
 }
-// starts[i], i <= kLineSeqs: where sequence i begins (wave 0 writes them).  Every
-// lane returns the line's length and the sequence that holds quantum `at`
-// (undefined beyond the end), for the piece's own start and length.
+// Lane i = sequence i; wave 0 (`write`) writes the line.  Returns the line's length,
+// that of a piece, and the sequence that the piece begins in.
 template <int QS>
-__device__ __forceinline__ int line(const TreeIn& a, int piece, int lane, bool write, int32_t* starts,
-                                    int& length, int& first) {
-  int q[4], sum = 0;
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    q[k] = 4 * lane + k < a.B ? quanta<QS>(a, 4 * lane + k) : 0;
-    sum += q[k];
-  }
-  int upto = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(upto, o);
-    if (lane >= o) upto += t;
-  }
+__device__ __forceinline__ int lay_line(const TreeIn& a, int piece, int lane, bool write, Line& line,
+                                        int& length, int& first) {
+  int p0 = 0, n = 0;
+  if (lane < a.B) n = tree_size(a.pos0, a.n_nodes, a.rows, lane, p0);
+  const int q = n > 0 ? 1 + (min(p0, a.C) + QS - 1) / QS : 0;
+  int upto = dpp_add<0x111, 0xF>(q);    // row_shr:1, :2, :4, :8
+  upto = dpp_add<0x112, 0xF>(upto);
+  upto = dpp_add<0x114, 0xF>(upto);
+  upto = dpp_add<0x118, 0xF>(upto);
+  upto = dpp_add<0x142, 0xA>(upto);     // row_bcast:15 and :31
+  upto = dpp_add<0x143, 0xC>(upto);
   const int total = __builtin_amdgcn_readlane(upto, 63);
+  if (write) {
+    line.starts[lane] = upto - q;
+    line.p0[lane] = p0;
+    line.n[lane] = n;
+    if (lane == 63) line.starts[kLineSeqs] = total;
+  }
   length = max(1, (total + a.pieces - 1) / a.pieces);
   const int at = piece * length;
-  int s = upto - sum, mine = 0;
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    if (write) starts[4 * lane + k] = s;
-    if (at >= s && at < s + q[k]) mine = 4 * lane + k;
-    s += q[k];
-  }
-  if (write && lane == 63) starts[kLineSeqs] = total;
-  const uint64_t who = __ballot(at >= upto - sum && at < upto);
-  first = who ? __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)who) - 1) : 0;
+  const uint64_t who = __ballot(at >= upto - q && at < upto);
+  first = who ? __ffsll((unsigned long long)who) - 1 : 0;
   return total;
 }
 // A workgroup's states of its place 0 or 1.
@@ -315,26 +313,31 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
   constexpr int QP = HD + 4;                  // floats per q row in LDS
   constexpr int DP = ROWB + 16;               // bytes per drafted row in LDS
   constexpr int FOLD = kTreeWaves * 16 * PART;
-  __shared__ __align__(16) float sq[NN * QP > FOLD ? NN * QP : FOLD];
+  constexpr int NSQ = NN * QP > FOLD ? NN * QP : FOLD;
+  __shared__ __align__(16) float sq[NSQ];
   __shared__ __align__(16) char sdk[DR * DP], sdv[DR * DP];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the G groups of one piece are 8 workgroups apart: on one XCD, reading alike
+  // All pieces of the first group of nodes, then all of the second: a multiple of
+  // 8 apart, a piece's two are on one XCD, reading alike.  (8 apart themselves, the
+  // first group, which has the more nodes, fell to every other CU.)
   constexpr int QS = kTreeWaves * SB;
-  const int group = G == 1 ? 0 : blockIdx.x / 8 % G;
-  const int share = G == 1 ? blockIdx.x : blockIdx.x / (8 * G) * 8 + blockIdx.x % 8;
+  const int shares = G == 1 ? gridDim.x : gridDim.x / G;
+  const int group = G == 1 ? 0 : blockIdx.x / shares, share = blockIdx.x - group * shares;
   const int piece = share / H, head = share % H;
   const int node0 = group * NN;  // this group's first node
-  __shared__ int32_t starts[kLineSeqs + 1], flag[kTreeWaves];
+  __shared__ Line line;
+  __shared__ int32_t flag[kTreeWaves];
   int first = piece, end = a.B, from = 0, to = 0;  // the piece: quanta [from, to) from sequence `first` on
   if (a.pieces) {
     if (G > 1 && piece >= a.pieces) return;
     int length;
-    const int total = line<QS>(a, piece, lane, wave == 0, starts, length, first);
+    const int total = lay_line<QS>(a, piece, lane, wave == 0, line, length, first);
     __syncthreads();
     if (blockIdx.x == 0) {  // for the merge
-      for (int i = threadIdx.x; i <= kLineSeqs; i += 64 * kTreeWaves) a.plan[i] = starts[i];
-      if (threadIdx.x == 0) a.plan[kLineSeqs + 1] = length;
+      for (int i = threadIdx.x; i <= kLineSeqs; i += 64 * kTreeWaves) a.plan[i] = line.starts[i];
+      if (threadIdx.x < kLineSeqs) a.plan[kLineSeqs + 1 + threadIdx.x] = line.n[threadIdx.x];
+      if (threadIdx.x == 0) a.plan[2 * kLineSeqs + 1] = length;
     }
     from = piece * length;
     to = min(total, from + length);
@@ -350,79 +353,62 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
   const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int32_t par = a.parent[(int64_t)b * a.rows + min(lane, a.rows - 1)];
-  int p0;
-  int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
-  n = __builtin_amdgcn_readfirstlane(n);
+  int p0, n;
+  if (a.pieces) {
+    p0 = line.p0[b];
+    n = line.n[b];
+  } else {
+    n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
+  }
   p0 = __builtin_amdgcn_readfirstlane(p0);
+  n = __builtin_amdgcn_readfirstlane(n);
+  if (n <= node0) continue;  // the whole workgroup
+  const int32_t par = a.parent[(int64_t)b * a.rows + min(lane, a.rows - 1)];
   const int nvalid = min(p0, a.C);
   int lo = 0, hi = nvalid;  // this workgroup's slots of the window
   bool drafts = true;       // and whether it has the drafted rows
   float* part = nullptr;    // where its states go; null: it has the whole sequence
   if (a.pieces) {
-    const int s0 = __builtin_amdgcn_readfirstlane(starts[b]), s1 = __builtin_amdgcn_readfirstlane(starts[b + 1]);
+    const int s0 = __builtin_amdgcn_readfirstlane(line.starts[b]),
+              s1 = __builtin_amdgcn_readfirstlane(line.starts[b + 1]);
     if (s0 >= to) break;
-    if (s0 == s1) continue;
     const int j0 = max(from - s0, 0), j1 = min(to, s1) - s0;
     drafts = j0 == 0;
     lo = max(j0 - 1, 0) * QS;
     hi = min(nvalid, (j1 - 1) * QS);
     if (s0 < from || s1 > to) part = states(a, share, group, G, min(a.rows, NN), s0 < from ? 0 : 1);
   }
-  if (n <= node0) continue;
-  const int tiles = min(NT, (n - node0 + 15) / 16);
   const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
   const char *kb = a.k + off, *vb = a.v + off;
   const int32_t* sp = a.sp + (int64_t)b * a.C;
 
   // The nodes' rows: q of this group's, and with the drafted rows K and V of every
-  // node that they may descend from; 32 rows at a time, thread -> row i / 8, dims
-  // 8 (i % 8) on.  Loads return in the order they are issued, so these go before
-  // the window's.
-  const int keys = drafts ? min((min(n, node0 + NN) + SB - 1) / SB * SB, DR) : 0;  // in batches
-  int row0 = keys ? 0 : node0;
-  const int d0 = (tid & 7) * 8;
-  const uint64_t anc = ancestors(par, n, lane);
-  float rq[8], rk[8], rv[8];
-  float2 cs[4];
-  auto load_rows = [&]() {
-    const int src = min(row0 + (tid >> 3), n - 1);
-    const int64_t roff = ((int64_t)b * a.rows + src) * a.row_stride + head * HD + d0;
-    if (a.qkv_bf16) {
-      load8<true>(a.qkv, roff, rq);
-      load8<true>(a.qkv, roff + D, rk);
-      load8<true>(a.qkv, roff + 2 * D, rv);
-    } else {
-      load8<false>(a.qkv, roff, rq);
-      load8<false>(a.qkv, roff + D, rk);
-      load8<false>(a.qkv, roff + 2 * D, rv);
-    }
-    const uint32_t al = __shfl((uint32_t)anc, src), ah = __shfl((uint32_t)(anc >> 32), src);
-    rope4_cs<true>(a.rope, p0 + __popc(al) + __popc(ah) - 1, d0, cs);
+  // node that they may descend from; thread -> row i / 8, dims 8 (i % 8) on.  The
+  // angles of the positions p0 .. p0 + 31, whichever of them the tree has.  Loads
+  // return in the order they are issued, so these go before the window's, and
+  // none waits for another.  (Angles read once the nodes' depths were known, and the
+  // position and count once more per sequence: three trips to memory, 7 us of
+  // the 12 that 8 voices' workgroups took.)
+  const int row0 = drafts ? 0 : node0, at_row = tid >> 3, d0 = (tid & 7) * 8;
+  const bool two = G > 1 && row0 < node0;  // the second group's keys begin with the first's rows
+  float rq[8] = {}, rk[8] = {}, rv[8] = {}, rk0[G > 1 ? 8 : 1] = {}, rv0[G > 1 ? 8 : 1] = {};
+  auto load_row = [&](int row, int part, float* r) {
+    const int64_t roff = ((int64_t)b * a.rows + min(row, a.rows - 1)) * a.row_stride + part * D + head * HD + d0;
+    if (a.qkv_bf16) load8<true>(a.qkv, roff, r);
+    else load8<false>(a.qkv, roff, r);
   };
-  auto store_rows = [&]() {
-    const int node = row0 + (tid >> 3);
-    if (node >= node0 && node < node0 + NN) {
-      rope8(cs, rq);
-#pragma unroll
-      for (int j = 0; j < 8; j++) sq[(node - node0) * QP + d0 + j] = rq[j] * 0.125f;  // exact
-    }
-    if (node < keys) {
-      rope8(cs, rk);
-      if (node >= n)
-#pragma unroll
-        for (int j = 0; j < 8; j++) rk[j] = rv[j] = 0.f;
-      store8<KV_BF16>(sdk + node * DP, d0, rk);
-      store8<KV_BF16>(sdv + node * DP, d0, rv);
-    }
-  };
-  static_assert(NN <= 8 * kTreeWaves, "a group's rows are read at once");
-  if (G > 1 && row0 < node0) {  // the second group's keys begin with the first's rows
-    load_rows();
-    store_rows();
-    row0 = node0;
+  load_row(node0 + at_row, 0, rq);
+  if (drafts) {
+    load_row(node0 + at_row, 1, rk);
+    load_row(node0 + at_row, 2, rv);
   }
-  load_rows();
+  if constexpr (G > 1)
+    if (two) {
+      load_row(at_row, 1, rk0);
+      load_row(at_row, 2, rv0);
+    }
+  float2 cs[4];
+  rope4_cs<true>(a.rope, p0 + at_row, d0, cs);
   __builtin_amdgcn_sched_barrier(0);
 
   TreeBatch<KV_BF16> x;
@@ -458,7 +444,46 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
   load_v(s0);
   __builtin_amdgcn_sched_barrier(0);
 
-  store_rows();
+  const int tiles = min(NT, (n - node0 + 15) / 16);
+  const int keys = drafts ? min((min(n, node0 + NN) + SB - 1) / SB * SB, DR) : 0;  // drafted rows, in batches
+  const uint64_t anc = ancestors(par, n, lane);
+  // the angles, by depth: in the part of sq that q leaves
+  static_assert(NN <= 8 * kTreeWaves && NN * QP + 32 * HD <= NSQ, "a group's rows are read at once");
+  float* const angles = sq + NN * QP;
+#pragma unroll
+  for (int j = 0; j < 4; j++) *(float2*)(angles + at_row * HD + d0 + 2 * j) = cs[j];
+  __syncthreads();
+  auto cs_of = [&](int node) {
+    const int src = min(node, n - 1);
+    const uint32_t al = __shfl((uint32_t)anc, src), ah = __shfl((uint32_t)(anc >> 32), src);
+    const int depth = __popc(al) + __popc(ah) - 1;
+    if (G == 1 || depth < 32) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) cs[j] = *(const float2*)(angles + (depth & 31) * HD + d0 + 2 * j);
+    } else {
+      rope4_cs<true>(a.rope, p0 + depth, d0, cs);
+    }
+  };
+  auto store_kv = [&](int node, float (&k)[8], float (&v)[8]) {
+    rope8(cs, k);
+    if (node >= n)
+#pragma unroll
+      for (int j = 0; j < 8; j++) k[j] = v[j] = 0.f;
+    store8<KV_BF16>(sdk + node * DP, d0, k);
+    store8<KV_BF16>(sdv + node * DP, d0, v);
+  };
+  cs_of(node0 + at_row);
+  if (at_row < NN) {
+    rope8(cs, rq);
+#pragma unroll
+    for (int j = 0; j < 8; j++) sq[at_row * QP + d0 + j] = rq[j] * 0.125f;  // exact
+  }
+  if (node0 + at_row < keys) store_kv(node0 + at_row, rk, rv);
+  if constexpr (G > 1)
+    if (two) {
+      cs_of(at_row);
+      store_kv(at_row, rk0, rv0);
+    }
   auto ancestors_of = [&](int t) {
     const int node = node0 + 16 * t + c;
     const uint32_t al = __shfl((uint32_t)anc, node), ah = __shfl((uint32_t)(anc >> 32), node);
@@ -710,9 +735,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
 __global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a, int groups) {
   const int b = blockIdx.x / H, head = blockIdx.x % H;
   const int lane = threadIdx.x & 63, g = lane >> 4, d = (lane & 15) * 4;
-  const int s = a.plan[b], e = a.plan[b + 1], length = a.plan[kLineSeqs + 1];
-  int p0;
-  const int n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
+  const int s = a.plan[b], e = a.plan[b + 1], n = a.plan[kLineSeqs + 1 + b], length = a.plan[2 * kLineSeqs + 1];
   const int node = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (node >= n || e == s) return;
   const int first = s / length, splits = (e - 1) / length - first + 1;
@@ -763,12 +786,15 @@ __global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a, int groups) 
 }
 
 // Workgroups per head of a launch whose work is cut as a line: with the groups
-// and heads as many as fit the chip at once (three per CU).  0: as many sequences
-// as fill the chip by themselves.
+// and heads two per CU.  (us for 24 voices of up to 61 nodes in fp32 / 3 of 64 over
+// 16384 slots / 8 of 16 over 2048, bf16: one per CU 57.2 / 55.4 / 17.3, two 57.1 /
+// 48.0 / 17.8, three, as many as fit, 61.1 / 49.3 / 18.2.)  0: as many sequences as
+// that by themselves, a workgroup for each.  (64 voices of 16 nodes: 61 us, as a
+// line of 64 pieces 75, two sequences' starts to a workgroup.)
 static int tree_groups(int rows) { return rows <= 32 ? 1 : 2; }
 static int tree_pieces(const mb_ctx* ctx, int B, int rows) {
   const int cus = ctx->cus_per_xcd > 0 ? ctx->xcds * ctx->cus_per_xcd : 256;
-  const int pieces = std::max(1, 3 * cus / (H * tree_groups(rows)));
+  const int pieces = std::max(1, 2 * cus / (H * tree_groups(rows)));
   return B < pieces && B <= kLineSeqs ? pieces : 0;
 }
 
