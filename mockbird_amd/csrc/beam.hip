@@ -598,6 +598,9 @@ int launch_beam_select(mb_ctx* ctx, int B, int W, int V, int n, const void* logi
   a.seen_out = seen_out;
   a.part = (char*)work;
   beam_parts(V, a.chunks, a.chunk);
+  // (a grid's work-items are counted in 32 bits)
+  if (((int64_t)B * W * a.chunks + 3) / 4 > INT32_MAX / 256 || (int64_t)B * 64 * kBeamWaves > INT32_MAX)
+    return fail(ctx, MB_ERR_ARG, "too many rows in one call");
   const dim3 block(64 * std::min(W, kBeamWaves));
   if (a.chunks == 1) {
     hipLaunchKernelGGL(k_beam_pick<true>, dim3((unsigned)B), block, 0, ctx->stream, a);
@@ -701,7 +704,7 @@ int launch_ring_reorder(mb_ctx* ctx, int layer0, int n_layers, int B, int W, con
   const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(max_rows, ring.C));
   const int64_t bx = (int64_t)n_layers * a.groups * H;
   const int64_t by = std::min<int64_t>(65535, (rows * row_chunks + 255) / 256);
-  if (bx > INT32_MAX) return fail(ctx, MB_ERR_ARG, "too many rings in one call");
+  if (bx > INT32_MAX / 256) return fail(ctx, MB_ERR_ARG, "too many rings in one call");
   const dim3 grid((unsigned)bx, (unsigned)by);
   auto go = [&](auto mw) {
     hipLaunchKernelGGL(k_ring_reorder<decltype(mw)::value>, grid, dim3(256), 0, ctx->stream, a, chunk_bits);

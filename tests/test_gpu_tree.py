@@ -79,6 +79,58 @@ def test_tree_attention_split_and_many(name, kv, B, T, C):
 
 
 @pytest.mark.parametrize("name,kv", KV)
+@pytest.mark.parametrize("B,T", [(20, 40), (21, 33), (22, 64), (41, 17), (42, 16), (43, 5), (65, 2)])
+def test_tree_attention_as_sequences_and_as_a_line(name, kv, B, T):
+    """Around the numbers of sequences from which each has workgroups of its own;
+    windows of all lengths, several sequences without nodes or rows."""
+    say(f"tree B={B} T={T} kv={name}")
+    rng = np.random.default_rng([B, T])
+    C = 90
+    pos0 = rng.integers(0, 3 * C, B).astype(np.int32)
+    pos0[rng.integers(0, B, 3)] = 0
+    n = rng.integers(0, T + 1, B).astype(np.int32)
+    n[rng.integers(0, B, 4)] = 0
+    with mb.Context(n_layers=1, capacity=C, max_seqs=B, max_rows=64, kv_dtype=kv) as ctx:
+        _fill(ctx, rng, 0, pos0)
+        qkv = rng.standard_normal((B, T, QKV), dtype=np.float32)
+        parent = random_parents(rng, B, T)
+        got = ctx.tree_attention(0, qkv, parent, pos0, n)
+        _check(ctx, 0, got, qkv, parent, pos0, n, kv == mb.MB_KV_BF16)
+        n[:] = 0  # nothing at all
+        out = np.full((B, T, D), 5.0, np.float32)
+        assert (ctx.tree_attention(0, qkv, parent, pos0, n, out) == 5.0).all()
+
+
+@pytest.mark.parametrize("B", [3, 70])
+def test_tree_device_positions_that_do_not_fit(B):
+    """Sequences at positions below 0 or above 2^31 - 65, and negative and too large
+    counts, on the device: left out, or taken to rows_max."""
+    import torch
+    rng = np.random.default_rng(14)
+    T, C = 6, 40
+    pos0 = rng.integers(0, 80, B).astype(np.int32)
+    n = np.full(B, T, np.int32)
+    n[1] = 2 ** 31 - 1
+    good = np.ones(B, bool)
+    for b, (p, m) in ((0, (-1, T)), (2, (2 ** 31 - 64, T)), (B - 2, (7, -5)), (B - 1, (-2 ** 31, T))):
+        pos0[b], n[b], good[b] = p, m, False
+    with mb.Context(n_layers=1, capacity=C, max_seqs=B, max_rows=64) as ctx:
+        _fill(ctx, rng, 0, np.where(good, pos0, 0))
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        rows = rng.standard_normal((B, T, QKV), dtype=np.float32)
+        parent = random_parents(rng, B, T)
+        q, w, p, c = (torch.from_numpy(x).cuda() for x in (rows, parent, pos0, n))
+        out = torch.full((B, T, D), 3.0, device="cuda")
+        _dev(ctx, 0, q, w, p, c, 2 ** 31 - 1, out)
+        got = out.cpu().numpy()
+        at = np.flatnonzero(good)
+        assert (got[~good] == 3.0).all()
+        for b in at:
+            want, bound = tree_reference(ctx.read_ring(0, b), rows[b], parent[b], int(pos0[b]), T, False)
+            assert (np.abs(got[b] - want) <= bound).all(), b
+
+
+@pytest.mark.parametrize("name,kv", KV)
 def test_tree_equals_appending_its_paths(name, kv):
     """Every node's output is what mb_append_attend ends with when its path is
     appended row by row: the window evicts alike.  Both are within their bounds

@@ -190,6 +190,7 @@ def beam_dev(h, B=2, W=4, V=100, n=4, logits=P, dtype=0, stride=100, scores=P, d
     (dict(V=5000, stride=5000, work=None), "workspace"),
     (dict(V=5000, stride=5000, work_bytes=64), "workspace"),
     (dict(V=5000, stride=5000, work=P + 8), "workspace"),
+    (dict(B=2 ** 31 - 1), "too many rows"),
 ])
 def test_beam_select_dev_refuses(bare, kw, words):
     h = bare()
@@ -225,6 +226,11 @@ def test_ring_reorder_dev_refuses(bare, kw, words):
     _refused(h, reorder_dev(h, **kw), mb.MB_ERR_ARG, words)
     assert reorder_dev(h, B=0, parent=None) == mb.MB_OK
     assert reorder_dev(h, most=0, parent=None) == mb.MB_OK
+
+
+def test_ring_reorder_of_more_rings_than_a_launch_takes(bare):
+    h = bare(n_layers=64, max_seqs=65535)
+    _refused(h, reorder_dev(h, L=64, B=65535, W=1), mb.MB_ERR_ARG, "too many rings")
 
 
 @pytest.mark.parametrize("a,z,code", [(-1, 5, mb.MB_ERR_ARG), (6, 5, mb.MB_ERR_ARG), (90, 101, mb.MB_ERR_RANGE)])
