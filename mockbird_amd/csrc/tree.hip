@@ -788,19 +788,27 @@ __global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a, int groups) 
 // Workgroups per head of a launch whose work is cut as a line: with the groups
 // and heads two per CU.  (us for 24 voices of up to 61 nodes in fp32 / 3 of 64 over
 // 16384 slots / 8 of 16 over 2048, bf16: one per CU 57.2 / 55.4 / 17.3, two 57.1 /
-// 48.0 / 17.8, three, as many as fit, 61.1 / 49.3 / 18.2.)  0: as many sequences as
-// that by themselves, a workgroup for each.  (64 voices of 16 nodes: 61 us, as a
-// line of 64 pieces 75, two sequences' starts to a workgroup.)
+// 48.0 / 17.8, three, as many as fit, 61.1 / 49.3 / 18.2.)  0: a workgroup for each
+// sequence, where a piece would not be shorter than the longest window by
+// kLineGain quanta, which is what the second launch and the sequences that begin
+// inside a piece cost.  (us as sequences / as a line, by voices x nodes x slots of
+// full quanta: 1 x 8 x 1024 fp32 17.5 / 9.4, 4 x 32 x 512 fp32 17.0 / 12.8, 8 x 16 x 2048
+// bf16 20.2 / 19.1, 10 x 2 x 1139 bf16 14.0 / 15.6, 16 x 16 x 1024 bf16 13.8 / 19.2, 30 x 16
+// x 1000 bf16 21.7 / 25.7, 12 x 48 x 700 bf16 17.1 / 25.0, 64 x 16 x 2048 bf16 61 / 75.)
+constexpr int kLineGain = 6;
 static int tree_groups(int rows) { return rows <= 32 ? 1 : 2; }
-static int tree_pieces(const mb_ctx* ctx, int B, int rows) {
+static int tree_pieces(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
   const int cus = ctx->cus_per_xcd > 0 ? ctx->xcds * ctx->cus_per_xcd : 256;
   const int pieces = std::max(1, 2 * cus / (H * tree_groups(rows)));
-  return B < pieces && B <= kLineSeqs ? pieces : 0;
+  const int qs = kTreeWaves * (ctx->cfg.kv_dtype == MB_KV_BF16 ? 32 : 16);
+  const int window = (std::min(max_pos, ctx->cfg.capacity) + qs - 1) / qs;
+  const int piece = (int)(((int64_t)B * (1 + window) + pieces - 1) / pieces);
+  return B <= kLineSeqs && window - piece >= kLineGain ? pieces : 0;
 }
 
-int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t) {
+int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
   if (B < 1) return 0;
-  const int64_t g = tree_groups(rows), p = tree_pieces(ctx, B, rows);
+  const int64_t g = tree_groups(rows), p = tree_pieces(ctx, B, rows, max_pos);
   return p ? 4 * (kPlanWords + p * H * g * 2 * std::min(rows, 32) * PART) : 0;
 }
 
@@ -825,7 +833,7 @@ int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, co
   a.out = out;
   a.out_stride = out_stride;
   a.B = B;
-  a.pieces = tree_pieces(ctx, B, rows);
+  a.pieces = tree_pieces(ctx, B, rows, max_pos);
   a.plan = (int32_t*)work;
   a.part = (float*)work + kPlanWords;
   const int groups = tree_groups(rows);
