@@ -322,7 +322,8 @@ struct BeamIn {
   int32_t *parent, *token, *done_out;
   uint32_t* seen_out;  // [B][n][words] or null
   char* part;          // chunks > 1: [B * W][chunks] PartRow
-  int chunks, chunk;   // parts of a row, ids of a part
+  int chunks, chunk;   // parts of a row in the workspace, ids of a part
+  int parts;           // parts of a row within its voice's workgroup (chunks 1)
 };
 
 // One part of a row, in the workspace: 16 bytes, then n (value, id) pairs.
@@ -370,6 +371,13 @@ __global__ __launch_bounds__(256) void k_beam_scan(const BeamIn a, int64_t parts
   if (lane < a.n) ((uint2*)(p + sizeof(PartRow)))[lane] = make_uint2(__float_as_uint(t.v), t.id);
 }
 
+// The maximum and sum of a row's parts, one to a lane (h.m = -inf elsewhere).
+__device__ __forceinline__ void join_sums(const PartRow& h, RowTop& t) {
+  t.m = wave_max(h.m);
+  // (an infinite maximum is the maximum of a part only where it was reached)
+  const double by = h.m == t.m ? 1.0 : (double)__expf(h.m - t.m);
+  t.sum = wave_sum(h.sum * by);
+}
 // The parts of a row joined.  Everything is read before anything is used.
 __device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, uint64_t* buf, RowTop& t) {
   PartRow h{0.0, -INFINITY, 0u};
@@ -392,10 +400,7 @@ __device__ __forceinline__ void join(const BeamIn& a, int64_t row, int lane, uin
     }
     take_top(z, [&](int j) { return ids[j]; }, a.n, lane, buf, t);
   }
-  t.m = wave_max(h.m);
-  // (an infinite maximum is the maximum of a part only where it was reached)
-  const double by = h.m == t.m ? 1.0 : (double)__expf(h.m - t.m);
-  t.sum = wave_sum(h.sum * by);
+  join_sums(h, t);
 }
 
 // The n best of `all` <= 64 J keys in LDS, the lower index first on equal ones,
@@ -485,29 +490,73 @@ __global__ __launch_bounds__(64 * kBeamWaves) void k_beam_pick(const BeamIn a) {
   __shared__ __align__(16) uint64_t buf[kBeamWaves][66];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int b = blockIdx.x, n = a.n;
-  for (int w = wave; w < a.W; w += nw) {
-    const int64_t row = (int64_t)b * a.W + w;
-    const float score = a.scores[row];
-    // (the row is read whether its beam has ended or not: waiting for the flag
-    // would cost every row a trip to memory)
-    const bool ended = a.done && a.done[row];
-    RowTop t;
-    if (FUSED) scan(a, row, 0, a.V, lane, buf[wave], t);
-    else join(a, row, lane, buf[wave], t);
+  auto put = [&](int at, const RowTop& t) {
+    if (lane < n) {
+      lv[at * n + lane] = t.v;
+      li[at * n + lane] = t.id;
+    }
+  };
+  auto finish = [&](int w, RowTop& t, float score, bool ended) {
     if (ended) {  // as a row of one id, whose logarithm is 0
       t.m = 0.f;
       t.sum = 1.0;
       t.v = lane == 0 ? 0.f : -INFINITY;
       t.id = lane == 0 ? (uint32_t)a.end_id : kNoId;
     }
-    if (lane < n) {
-      lv[w * n + lane] = t.v;
-      li[w * n + lane] = t.id;
-    }
+    put(w, t);
     if (lane == 0) {
       lm[w] = t.m;
       ls[w] = log(t.sum);
       sc[w] = (double)score;
+    }
+  };
+  // (a row is read whether its beam has ended or not: waiting for the flag would
+  // cost every row a trip to memory)
+  if (FUSED && a.parts > 1) {  // W parts <= kBeamWaves: a wave for each part
+    const int w = wave / a.parts, part = wave - w * a.parts;
+    const int64_t row = (int64_t)b * a.W + w, mine = (int64_t)b * a.W + min(wave, a.W - 1);
+    const float score = a.scores[mine];
+    const bool ended = a.done && a.done[mine];
+    RowTop t;
+    scan(a, row, part * a.chunk, min(a.V, (part + 1) * a.chunk), lane, buf[wave], t);
+    put(wave, t);
+    if (lane == 0) {
+      lm[wave] = t.m;
+      ls[wave] = t.sum;
+    }
+    __syncthreads();
+    // wave w < W joins row w's parts
+    const int all = a.parts * n;  // <= 512
+    PartRow h{0.0, -INFINITY, 0u};
+    float z[16];
+    uint32_t ids[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      const int i = 64 * j + lane;
+      const bool in = j < 8 && i < all && wave < a.W;
+      z[j] = in ? lv[wave * all + i] : -INFINITY;
+      ids[j] = in ? li[wave * all + i] : kNoId;
+    }
+    if (wave < a.W && lane < a.parts) {
+      h.m = lm[wave * a.parts + lane];
+      h.sum = ls[wave * a.parts + lane];
+    }
+    __syncthreads();
+    if (wave < a.W) {
+      t = RowTop{};
+      take_top(z, [&](int j) { return ids[j]; }, n, lane, buf[wave], t);
+      join_sums(h, t);
+      finish(wave, t, score, ended);
+    }
+  } else {
+    for (int w = wave; w < a.W; w += nw) {
+      const int64_t row = (int64_t)b * a.W + w;
+      const float score = a.scores[row];
+      const bool ended = a.done && a.done[row];
+      RowTop t;
+      if (FUSED) scan(a, row, 0, a.V, lane, buf[wave], t);
+      else join(a, row, lane, buf[wave], t);
+      finish(w, t, score, ended);
     }
   }
   __syncthreads();
@@ -559,17 +608,28 @@ __global__ __launch_bounds__(64 * kBeamWaves) void k_beam_pick(const BeamIn a) {
   }
 }
 
-// Ids of a row that one wave reads: all where the voice's own workgroup scans
-// its rows, else a 64th of the row at least.
-constexpr int kBeamFusedVocab = 4096;
-static void beam_parts(int V, int& chunks, int& chunk) {
-  chunk = V <= kBeamFusedVocab ? V : std::max(1, (V + 64 * kScan - 1) / (64 * kScan)) * kScan;
+// How a row is cut.  One launch, a workgroup per voice, where its waves can read
+// every row's 1024 ids at a time side by side (`parts` waves a row); else a scan by
+// a wave per part of a row, and the choice in a second launch.  (Rows of 2477, 3383
+// and 5489 ids of 14, 2 and 2 beams read by one wave each took 21.0, 12.8 and, in two
+// launches, 11.1 us.)
+static void beam_parts(int W, int V, int& chunks, int& chunk, int& parts) {
+  const int reads = (V + kScan - 1) / kScan;
+  chunks = parts = 1;
+  chunk = V;
+  if (reads == 1) return;
+  if ((int64_t)W * reads <= kBeamWaves) {
+    parts = reads;
+    chunk = kScan;
+    return;
+  }
+  chunk = (V + 64 * kScan - 1) / (64 * kScan) * kScan;
   chunks = (V + chunk - 1) / chunk;
 }
 
 int64_t beam_work_bytes(int B, int W, int V, int n) {
-  int chunks, chunk;
-  beam_parts(V, chunks, chunk);
+  int chunks, chunk, parts;
+  beam_parts(W, V, chunks, chunk, parts);
   return chunks > 1 ? (int64_t)B * W * chunks * (int64_t)(sizeof(PartRow) + n * 8) : 0;
 }
 
@@ -597,11 +657,11 @@ int launch_beam_select(mb_ctx* ctx, int B, int W, int V, int n, const void* logi
   a.done_out = done_out;
   a.seen_out = seen_out;
   a.part = (char*)work;
-  beam_parts(V, a.chunks, a.chunk);
+  beam_parts(W, V, a.chunks, a.chunk, a.parts);
   // (a grid's work-items are counted in 32 bits)
   if (((int64_t)B * W * a.chunks + 3) / 4 > INT32_MAX / 256 || (int64_t)B * 64 * kBeamWaves > INT32_MAX)
     return fail(ctx, MB_ERR_ARG, "too many rows in one call");
-  const dim3 block(64 * std::min(W, kBeamWaves));
+  const dim3 block(64 * std::min(W * a.parts, kBeamWaves));
   if (a.chunks == 1) {
     hipLaunchKernelGGL(k_beam_pick<true>, dim3((unsigned)B), block, 0, ctx->stream, a);
   } else {
