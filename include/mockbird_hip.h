@@ -266,8 +266,8 @@ int mb_ring_view(mb_ctx* ctx, void** k, void** v, int32_t** slot_pos);
  *   - the slots of `layer` whose stored position p satisfies p < pos0[b] and
  *     lies in its window (0 <= its position - p < capacity): rows of an
  *     earlier draft at pos0[b] and later are not seen;
- *   - its ancestors' rows and its own, K roped at their positions, K and V
- *     rounded as the ring would store them.
+ *   - its ancestors' rows in that window and its own, K roped at their
+ *     positions, K and V rounded as the ring would store them.
  * out [B][rows_max][768] receives each node's attention output: what appending
  * its ancestors and it one by one (mb_append_attend) would end with, to
  * rounding.  Rows i >= n_nodes[b] of out are left as they are.  The rings are
@@ -284,7 +284,8 @@ int mb_tree_attention_work(mb_ctx* ctx, int B, int rows_max, int32_t max_pos, in
 /* Device-pointer form (enqueue only).  max_pos bounds every node's position
  * (a larger bound than needed is right too): it sizes the split of the windows.
  * n_nodes may be NULL (rows_max each).  qkv_stride and out_stride are in
- * elements between rows; every row starts at a multiple of 16 bytes.  A parent
+ * elements between rows; every row starts at a multiple of 16 bytes,
+ * and no row of out overlaps one of qkv.  A parent
  * that is not an earlier node counts as -1; a sequence whose positions do not
  * fit int32 (pos0[b] < 0 or > 2^31 - 65) is left out.  `work` holds
  * mb_tree_attention_work bytes, 16-byte aligned, of any content; calls that may
@@ -328,7 +329,7 @@ int mb_tree_commit_dev(mb_ctx* ctx, int layer0, int n_layers, int B, int rows_ma
  * Where fewer continuations exist: -inf, -1, -1, 1 and an empty set.
  * width and n_out are 1 .. 32.  done may be NULL (none), and then end_id may
  * be -1 (no id ends a beam); seen may be NULL (no penalty), and then seen_out
- * is NULL.  Outputs may not be the inputs. */
+ * is NULL.  Outputs may not overlap inputs. */
 int mb_beam_select(mb_ctx* ctx, int B, int width, int vocab, int n_out, const float* logits,
                    const float* scores, const int32_t* done, int32_t end_id, const uint32_t* seen,
                    double penalty, float* scores_out, int32_t* parent, int32_t* token,

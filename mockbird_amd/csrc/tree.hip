@@ -8,8 +8,8 @@
 //     p_i - p < C: what the window would hold had its ancestors been appended
 //     (their appends evict exactly the positions p <= p_i - C), and nothing of
 //     an earlier draft that was not kept (p >= pos0);
-//   - the drafted rows of its ancestors and its own, K roped at their own
-//     positions and K and V rounded as the ring stores them.
+//   - the drafted rows of its ancestors in its window (p_i - p < C) and its own, K
+//     roped at their own positions and K and V rounded as the ring stores them.
 // So out_i is what appending i's ancestors and i one after another and then
 // attending would give, for all nodes in one pass over the window.
 #include <algorithm>
@@ -287,7 +287,8 @@ __device__ __forceinline__ void exact_rows(const TreeIn& a, int tid, int b, int 
       const bool live = p >= 0 && p < p0 && (int64_t)pos - p < a.C;
       if (__ballot(live)) rows(kb + (int64_t)base * HD * E, vb + (int64_t)base * HD * E, HD * E, live);
     }
-    if (drafts) rows(dk, dv, dpitch, lane < n && ((mine >> lane) & 1));
+    if (drafts)
+      rows(dk, dv, dpitch, lane < n && ((mine >> lane) & 1) && __popcll(mine) - __popcll(anc) < a.C);
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
     if (part) {
       float* pp = part + (node - node0) * PART;
@@ -348,305 +349,310 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
   }
 
   for (int b = first; b < end; b++) {
-  // (the thread's places are worked out anew for each sequence: kept over the
-  // loop they would take more registers than there are)
-  int tid = threadIdx.x;
-  asm volatile("" : "+v"(tid));
-  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-  int p0, n;
-  if (a.pieces) {
-    p0 = line.p0[b];
-    n = line.n[b];
-  } else {
-    n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
-  }
-  p0 = __builtin_amdgcn_readfirstlane(p0);
-  n = __builtin_amdgcn_readfirstlane(n);
-  if (n <= node0) continue;  // the whole workgroup
-  const int32_t par = a.parent[(int64_t)b * a.rows + min(lane, a.rows - 1)];
-  const int nvalid = min(p0, a.C);
-  int lo = 0, hi = nvalid;  // this workgroup's slots of the window
-  bool drafts = true;       // and whether it has the drafted rows
-  float* part = nullptr;    // where its states go; null: it has the whole sequence
-  if (a.pieces) {
-    const int s0 = __builtin_amdgcn_readfirstlane(line.starts[b]),
-              s1 = __builtin_amdgcn_readfirstlane(line.starts[b + 1]);
-    if (s0 >= to) break;
-    const int j0 = max(from - s0, 0), j1 = min(to, s1) - s0;
-    drafts = j0 == 0;
-    lo = max(j0 - 1, 0) * QS;
-    hi = min(nvalid, (j1 - 1) * QS);
-    if (s0 < from || s1 > to) part = states(a, share, group, G, min(a.rows, NN), s0 < from ? 0 : 1);
-  }
-  const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
-  const char *kb = a.k + off, *vb = a.v + off;
-  const int32_t* sp = a.sp + (int64_t)b * a.C;
-
-  // The nodes' rows: q of this group's, and with the drafted rows K and V of every
-  // node that they may descend from; thread -> row i / 8, dims 8 (i % 8) on.  The
-  // angles of the positions p0 .. p0 + 31, whichever of them the tree has.  Loads
-  // return in the order they are issued, so these go before the window's, and
-  // none waits for another.  (Angles read once the nodes' depths were known, and the
-  // position and count once more per sequence: three trips to memory, 7 us of
-  // the 12 that 8 voices' workgroups took.)
-  const int row0 = drafts ? 0 : node0, at_row = tid >> 3, d0 = (tid & 7) * 8;
-  const bool two = G > 1 && row0 < node0;  // the second group's keys begin with the first's rows
-  float rq[8] = {}, rk[8] = {}, rv[8] = {}, rk0[G > 1 ? 8 : 1] = {}, rv0[G > 1 ? 8 : 1] = {};
-  auto load_row = [&](int row, int part, float* r) {
-    const int64_t roff = ((int64_t)b * a.rows + min(row, a.rows - 1)) * a.row_stride + part * D + head * HD + d0;
-    if (a.qkv_bf16) load8<true>(a.qkv, roff, r);
-    else load8<false>(a.qkv, roff, r);
-  };
-  load_row(node0 + at_row, 0, rq);
-  if (drafts) {
-    load_row(node0 + at_row, 1, rk);
-    load_row(node0 + at_row, 2, rv);
-  }
-  if constexpr (G > 1)
-    if (two) {
-      load_row(at_row, 1, rk0);
-      load_row(at_row, 2, rv0);
+    // (the thread's places are worked out anew for each sequence: kept over the
+    // loop they would take more registers than there are)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+    int p0, n;
+    if (a.pieces) {
+      p0 = line.p0[b];
+      n = line.n[b];
+    } else {
+      n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
     }
-  float2 cs[4];
-  rope4_cs<true>(a.rope, p0 + at_row, d0, cs);
-  __builtin_amdgcn_sched_barrier(0);
+    p0 = __builtin_amdgcn_readfirstlane(p0);
+    n = __builtin_amdgcn_readfirstlane(n);
+    if (n <= node0) continue;  // the whole workgroup
+    const int32_t par = a.parent[(int64_t)b * a.rows + min(lane, a.rows - 1)];
+    const int nvalid = min(p0, a.C);
+    int lo = 0, hi = nvalid;  // this workgroup's slots of the window
+    bool drafts = true;       // and whether it has the drafted rows
+    float* part = nullptr;    // where its states go; null: it has the whole sequence
+    if (a.pieces) {
+      const int s0 = __builtin_amdgcn_readfirstlane(line.starts[b]),
+                s1 = __builtin_amdgcn_readfirstlane(line.starts[b + 1]);
+      if (s0 >= to) break;
+      const int j0 = max(from - s0, 0), j1 = min(to, s1) - s0;
+      drafts = j0 == 0;
+      lo = max(j0 - 1, 0) * QS;
+      hi = min(nvalid, (j1 - 1) * QS);
+      if (s0 < from || s1 > to) part = states(a, share, group, G, min(a.rows, NN), s0 < from ? 0 : 1);
+    }
+    const int64_t off = ((int64_t)b * a.seq_stride + (int64_t)head * a.C * HD) * E;
+    const char *kb = a.k + off, *vb = a.v + off;
+    const int32_t* sp = a.sp + (int64_t)b * a.C;
 
-  TreeBatch<KV_BF16> x;
-  int32_t spl;  // lane l: the stored position of the batch's slot l % SB
-  // Slots past the window read its last one (slot 0 of an empty window) and
-  // are dead by their position.  (A head's run is at most 2^28 bytes.)
-  const int last = max(hi - 1, 0);
-  auto load_k = [&](int base) {
-    spl = sp[min(base + (lane & (SB - 1)), last)];
-    if constexpr (KV_BF16) {
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const char* r = kb + (uint32_t)(min(base + 16 * u + c, last) * ROWB + g * 16);
-#pragma unroll
-        for (int h = 0; h < 2; h++) x.k[2 * u + h] = ring_load<G == 1, u32x4_t>(r + 64 * h);
+    // The nodes' rows: q of this group's, and with the drafted rows K and V of every
+    // node that they may descend from; thread -> row i / 8, dims 8 (i % 8) on.  The
+    // angles of the positions p0 .. p0 + 31, whichever of them the tree has.  Loads
+    // return in the order they are issued, so these go before the window's, and
+    // none waits for another.  (Angles read once the nodes' depths were known, and the
+    // position and count once more per sequence: three trips to memory, 7 us of
+    // the 12 that 8 voices' workgroups took.)
+    const int row0 = drafts ? 0 : node0, at_row = tid >> 3, d0 = (tid & 7) * 8;
+    const bool two = G > 1 && row0 < node0;  // the second group's keys begin with the first's rows
+    float rq[8] = {}, rk[8] = {}, rv[8] = {}, rk0[G > 1 ? 8 : 1] = {}, rv0[G > 1 ? 8 : 1] = {};
+    auto load_row = [&](int row, int part, float* r) {
+      const int64_t roff = ((int64_t)b * a.rows + min(row, a.rows - 1)) * a.row_stride + part * D + head * HD + d0;
+      if (a.qkv_bf16) load8<true>(a.qkv, roff, r);
+      else load8<false>(a.qkv, roff, r);
+    };
+    load_row(node0 + at_row, 0, rq);
+    if (drafts) {
+      load_row(node0 + at_row, 1, rk);
+      load_row(node0 + at_row, 2, rv);
+    }
+    if constexpr (G > 1)
+      if (two) {
+        load_row(at_row, 1, rk0);
+        load_row(at_row, 2, rv0);
       }
-    } else {
-      const char* r = kb + (uint32_t)(min(base + c, last) * ROWB + g * 16);
-#pragma unroll
-      for (int q = 0; q < 4; q++) x.k[q] = ring_load<G == 1, u32x4_t>(r + 64 * q);
-    }
-  };
-  auto load_v = [&](int base) {
-#pragma unroll
-    for (int j = 0; j < NS; j++) {
-      const char* r = vb + (uint32_t)(min(base + 16 * (j >> 2) + 4 * g + (j & 3), last) * ROWB + c * 4 * E);
-      if constexpr (KV_BF16) x.v[j] = ring_load<G == 1, u32x2_t>(r);
-      else x.v[j] = ring_load<G == 1, u32x4_t>(r);
-    }
-  };
-  const int s0 = lo + wave * SB, step = kTreeWaves * SB;
-  load_k(s0);
-  load_v(s0);
-  __builtin_amdgcn_sched_barrier(0);
+    float2 cs[4];
+    rope4_cs<true>(a.rope, p0 + at_row, d0, cs);
+    __builtin_amdgcn_sched_barrier(0);
 
-  const int tiles = min(NT, (n - node0 + 15) / 16);
-  const int keys = drafts ? min((min(n, node0 + NN) + SB - 1) / SB * SB, DR) : 0;  // drafted rows, in batches
-  const uint64_t anc = ancestors(par, n, lane);
-  // the angles, by depth: in the part of sq that q leaves
-  static_assert(NN <= 8 * kTreeWaves && NN * QP + 32 * HD <= NSQ, "a group's rows are read at once");
-  float* const angles = sq + NN * QP;
-#pragma unroll
-  for (int j = 0; j < 4; j++) *(float2*)(angles + at_row * HD + d0 + 2 * j) = cs[j];
-  __syncthreads();
-  auto cs_of = [&](int node) {
-    const int src = min(node, n - 1);
-    const uint32_t al = __shfl((uint32_t)anc, src), ah = __shfl((uint32_t)(anc >> 32), src);
-    const int depth = __popc(al) + __popc(ah) - 1;
-    if (G == 1 || depth < 32) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) cs[j] = *(const float2*)(angles + (depth & 31) * HD + d0 + 2 * j);
-    } else {
-      rope4_cs<true>(a.rope, p0 + depth, d0, cs);
-    }
-  };
-  auto store_kv = [&](int node, float (&k)[8], float (&v)[8]) {
-    rope8(cs, k);
-    if (node >= n)
-#pragma unroll
-      for (int j = 0; j < 8; j++) k[j] = v[j] = 0.f;
-    store8<KV_BF16>(sdk + node * DP, d0, k);
-    store8<KV_BF16>(sdv + node * DP, d0, v);
-  };
-  cs_of(node0 + at_row);
-  if (at_row < NN) {
-    rope8(cs, rq);
-#pragma unroll
-    for (int j = 0; j < 8; j++) sq[at_row * QP + d0 + j] = rq[j] * 0.125f;  // exact
-  }
-  if (node0 + at_row < keys) store_kv(node0 + at_row, rk, rv);
-  if constexpr (G > 1)
-    if (two) {
-      cs_of(at_row);
-      store_kv(at_row, rk0, rv0);
-    }
-  auto ancestors_of = [&](int t) {
-    const int node = node0 + 16 * t + c;
-    const uint32_t al = __shfl((uint32_t)anc, node), ah = __shfl((uint32_t)(anc >> 32), node);
-    return (uint64_t)ah << 32 | al;
-  };
-  int deepest = lane < n ? __popcll(anc) - 1 : 0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o));
-  deepest = __builtin_amdgcn_readfirstlane(deepest);
-  __syncthreads();
-
-  // q as the second operand of the scores: in registers, or with two tiles of
-  // bf16 planes in LDS, in the lanes' order (48 registers less)
-  constexpr bool QLDS = KV_BF16 && NT > 1;
-  __shared__ uint4 sqp[QLDS ? NT * 2 : 1][3][QLDS ? 64 : 1];
-  std::conditional_t<KV_BF16, Planes[QLDS ? 1 : NT][2], f32x4_t[NT][4]> q;
-  auto planes = [&](int t, int h) {
-    const float* r = sq + (16 * t + c) * QP + 32 * h + 8 * g;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = r[j];
-    return split3(v);
-  };
-  if constexpr (QLDS) {
-    for (int i = wave; i < NT * 2; i += kTreeWaves) {
-      const Planes p = planes(i >> 1, i & 1);
-#pragma unroll
-      for (int k = 0; k < 3; k++) sqp[i][k][lane] = __builtin_bit_cast(uint4, p.p[k]);
-    }
-    __syncthreads();
-  } else {
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
+    TreeBatch<KV_BF16> x;
+    int32_t spl;  // lane l: the stored position of the batch's slot l % SB
+    // Slots past the window read its last one (slot 0 of an empty window) and
+    // are dead by their position.  (A head's run is at most 2^28 bytes.)
+    const int last = max(hi - 1, 0);
+    auto load_k = [&](int base) {
+      spl = sp[min(base + (lane & (SB - 1)), last)];
       if constexpr (KV_BF16) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) q[t][h] = planes(t, h);
+        for (int u = 0; u < 2; u++) {
+          const char* r = kb + (uint32_t)(min(base + 16 * u + c, last) * ROWB + g * 16);
+#pragma unroll
+          for (int h = 0; h < 2; h++) x.k[2 * u + h] = ring_load<G == 1, u32x4_t>(r + 64 * h);
+        }
       } else {
+        const char* r = kb + (uint32_t)(min(base + c, last) * ROWB + g * 16);
 #pragma unroll
-        for (int j = 0; j < 4; j++) q[t][j] = *(const f32x4_t*)(sq + (16 * t + c) * QP + 16 * j + 4 * g);
+        for (int q = 0; q < 4; q++) x.k[q] = ring_load<G == 1, u32x4_t>(r + 64 * q);
       }
-    }
-  }
-  auto plane = [&](auto& q, int t, int h, int k) {
-    if constexpr (QLDS) return __builtin_bit_cast(bf16x8_t, sqp[2 * t + h][k][lane]);
-    else return q[t][h].p[k];
-  };
-
-  TreeState<KV_BF16, NT> st;
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-#pragma unroll
-    for (int dt = 0; dt < 4; dt++) st.o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    st.m[t] = -INFINITY;
-    st.l[t] = 0.f;
-  }
-
-  // scores s[t][j] of slot 16 (j / 4) + 4g + j % 4 of the batch
-  float s[NT][NS];
-  auto scores = [&]() {
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-      if (NT > 1 && t >= tiles) break;  // uniform
-      if constexpr (KV_BF16) {
-        f32x4_t d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (int k = 2; k >= 0; k--)
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const bf16x8_t p = plane(q, t, h, k);
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-              d[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x.k[2 * u + h]), p,
-                                                             d[u], 0, 0, 0);
-          }
-#pragma unroll
-        for (int j = 0; j < 8; j++) s[t][j] = d[j >> 2][j & 3];
-      } else {
-        f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[j][e]), q[t][j][e], d, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 4; j++) s[t][j] = d[j];
-      }
-    }
-  };
-  // the batch's scores into the states
-  auto apply = [&]() {
-    bf16x8_t vt[4];
-    if constexpr (KV_BF16) {
-#pragma unroll
-      for (int dt = 0; dt < 4; dt++) {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          w[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][dt >> 1], x.v[2 * j][dt >> 1],
-                                       dt & 1 ? 0x07060302u : 0x05040100u);
-        vt[dt] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-      if (NT > 1 && t >= tiles) break;
-      float mx = s[t][0];
-#pragma unroll
-      for (int j = 1; j < NS; j++) mx = fmaxf(mx, s[t][j]);
-      mx = fmaxf(col_max(mx), st.m[t]);
-      if (__ballot(mx > st.m[t])) {  // uniform
-        const float by = mx == -INFINITY ? 1.f : __expf(st.m[t] - mx);
-        st.l[t] *= by;
-#pragma unroll
-        for (int dt = 0; dt < 4; dt++) st.o[t][dt] *= by;
-        st.m[t] = mx;
-      }
-      const float m = mx == -INFINITY ? 0.f : mx;
-      float p[NS];
+    };
+    auto load_v = [&](int base) {
 #pragma unroll
       for (int j = 0; j < NS; j++) {
-        p[j] = __expf(s[t][j] - m);
-        st.l[t] += p[j];
+        const char* r = vb + (uint32_t)(min(base + 16 * (j >> 2) + 4 * g + (j & 3), last) * ROWB + c * 4 * E);
+        if constexpr (KV_BF16) x.v[j] = ring_load<G == 1, u32x2_t>(r);
+        else x.v[j] = ring_load<G == 1, u32x4_t>(r);
       }
-      if constexpr (KV_BF16) {
-        const Planes pp = split3(p);
-#pragma unroll
-        for (int k = 2; k >= 0; k--)
-#pragma unroll
-          for (int dt = 0; dt < 4; dt++)
-            st.o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[dt], pp.p[k], st.o[t][dt], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int dt = 0; dt < 4; dt++)
-            st.o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][dt]), p[j],
-                                                               st.o[t][dt], 0, 0, 0);
-      }
-    }
-  };
+    };
+    const int s0 = lo + wave * SB, step = kTreeWaves * SB;
+    load_k(s0);
+    load_v(s0);
+    __builtin_amdgcn_sched_barrier(0);
 
-  for (int base = s0; base < hi; base += step) {
-    const int32_t sc = base + (lane & (SB - 1)) < hi ? spl : -1;
-    scores();
-    // (loaded past the last batch too, from the last slot: a branch around the
-    // loads would have the next wait drain them all)
-    load_k(base + step);
-    const uint64_t all = __ballot((sc >= 0) & (sc < p0) & (p0 + deepest - sc < a.C));
-    if (~all) {  // uniform
+    const int tiles = min(NT, (n - node0 + 15) / 16);
+    const int keys = drafts ? min((min(n, node0 + NN) + SB - 1) / SB * SB, DR) : 0;  // drafted rows, in batches
+    const uint64_t anc = ancestors(par, n, lane);
+    // the angles, by depth: in the part of sq that q leaves
+    static_assert(NN <= 8 * kTreeWaves && NN * QP + 32 * HD <= NSQ, "a group's rows are read at once");
+    float* const angles = sq + NN * QP;
+#pragma unroll
+    for (int j = 0; j < 4; j++) *(float2*)(angles + at_row * HD + d0 + 2 * j) = cs[j];
+    __syncthreads();
+    auto cs_of = [&](int node) {
+      const int src = min(node, n - 1);
+      const uint32_t al = __shfl((uint32_t)anc, src), ah = __shfl((uint32_t)(anc >> 32), src);
+      const int depth = __popc(al) + __popc(ah) - 1;
+      if (G == 1 || depth < 32) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) cs[j] = *(const float2*)(angles + (depth & 31) * HD + d0 + 2 * j);
+      } else {
+        rope4_cs<true>(a.rope, p0 + depth, d0, cs);
+      }
+    };
+    auto store_kv = [&](int node, float (&k)[8], float (&v)[8]) {
+      rope8(cs, k);
+      if (node >= n)
+#pragma unroll
+        for (int j = 0; j < 8; j++) k[j] = v[j] = 0.f;
+      store8<KV_BF16>(sdk + node * DP, d0, k);
+      store8<KV_BF16>(sdv + node * DP, d0, v);
+    };
+    cs_of(node0 + at_row);
+    if (at_row < NN) {
+      rope8(cs, rq);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sq[at_row * QP + d0 + j] = rq[j] * 0.125f;  // exact
+    }
+    if (node0 + at_row < keys) store_kv(node0 + at_row, rk, rv);
+    if constexpr (G > 1)
+      if (two) {
+        cs_of(at_row);
+        store_kv(at_row, rk0, rv0);
+      }
+    auto masks_of = [&](uint64_t mask, int t) {  // of node c of the tile
+      const int node = node0 + 16 * t + c;
+      const uint32_t lo = __shfl((uint32_t)mask, node), hi = __shfl((uint32_t)(mask >> 32), node);
+      return (uint64_t)hi << 32 | lo;
+    };
+    int deepest = lane < n ? __popcll(anc) - 1 : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o));
+    deepest = __builtin_amdgcn_readfirstlane(deepest);
+    __syncthreads();
+
+    // q as the second operand of the scores: in registers, or with two tiles of
+    // bf16 planes in LDS, in the lanes' order (48 registers less)
+    constexpr bool QLDS = KV_BF16 && NT > 1;
+    __shared__ uint4 sqp[QLDS ? NT * 2 : 1][3][QLDS ? 64 : 1];
+    std::conditional_t<KV_BF16, Planes[QLDS ? 1 : NT][2], f32x4_t[NT][4]> q;
+    auto planes = [&](int t, int h) {
+      const float* r = sq + (16 * t + c) * QP + 32 * h + 8 * g;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = r[j];
+      return split3(v);
+    };
+    if constexpr (QLDS) {
+      for (int i = wave; i < NT * 2; i += kTreeWaves) {
+        const Planes p = planes(i >> 1, i & 1);
+#pragma unroll
+        for (int k = 0; k < 3; k++) sqp[i][k][lane] = __builtin_bit_cast(uint4, p.p[k]);
+      }
+      __syncthreads();
+    } else {
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const int32_t at = p0 + __popcll(ancestors_of(t)) - 1;
+        if constexpr (KV_BF16) {
 #pragma unroll
-        for (int j = 0; j < NS; j++) {
-          const int32_t p = __shfl(sc, 16 * (j >> 2) + 4 * g + (j & 3));
-          s[t][j] = ((p >= 0) & (p < p0) & (at - p < a.C)) ? s[t][j] : -INFINITY;
+          for (int h = 0; h < 2; h++) q[t][h] = planes(t, h);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++) q[t][j] = *(const f32x4_t*)(sq + (16 * t + c) * QP + 16 * j + 4 * g);
         }
       }
     }
-    apply();
-    load_v(base + step);
-  }
-  {
+    auto plane = [&](auto& q, int t, int h, int k) {
+      if constexpr (QLDS) return __builtin_bit_cast(bf16x8_t, sqp[2 * t + h][k][lane]);
+      else return q[t][h].p[k];
+    };
+
+    TreeState<KV_BF16, NT> st;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+      for (int dt = 0; dt < 4; dt++) st.o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      st.m[t] = -INFINITY;
+      st.l[t] = 0.f;
+    }
+
+    // scores s[t][j] of slot 16 (j / 4) + 4g + j % 4 of the batch
+    float s[NT][NS];
+    auto scores = [&]() {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        if (NT > 1 && t >= tiles) break;  // uniform
+        if constexpr (KV_BF16) {
+          f32x4_t d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int k = 2; k >= 0; k--)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const bf16x8_t p = plane(q, t, h, k);
+#pragma unroll
+              for (int u = 0; u < 2; u++)
+                d[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x.k[2 * u + h]), p,
+                                                               d[u], 0, 0, 0);
+            }
+#pragma unroll
+          for (int j = 0; j < 8; j++) s[t][j] = d[j >> 2][j & 3];
+        } else {
+          f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[j][e]), q[t][j][e], d, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[t][j] = d[j];
+        }
+      }
+    };
+    // the batch's scores into the states
+    auto apply = [&]() {
+      bf16x8_t vt[4];
+      if constexpr (KV_BF16) {
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            w[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][dt >> 1], x.v[2 * j][dt >> 1],
+                                         dt & 1 ? 0x07060302u : 0x05040100u);
+          vt[dt] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        if (NT > 1 && t >= tiles) break;
+        float mx = s[t][0];
+#pragma unroll
+        for (int j = 1; j < NS; j++) mx = fmaxf(mx, s[t][j]);
+        mx = fmaxf(col_max(mx), st.m[t]);
+        if (__ballot(mx > st.m[t])) {  // uniform
+          const float by = mx == -INFINITY ? 1.f : __expf(st.m[t] - mx);
+          st.l[t] *= by;
+#pragma unroll
+          for (int dt = 0; dt < 4; dt++) st.o[t][dt] *= by;
+          st.m[t] = mx;
+        }
+        const float m = mx == -INFINITY ? 0.f : mx;
+        float p[NS];
+#pragma unroll
+        for (int j = 0; j < NS; j++) {
+          p[j] = __expf(s[t][j] - m);
+          st.l[t] += p[j];
+        }
+        if constexpr (KV_BF16) {
+          const Planes pp = split3(p);
+#pragma unroll
+          for (int k = 2; k >= 0; k--)
+#pragma unroll
+            for (int dt = 0; dt < 4; dt++)
+              st.o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[dt], pp.p[k], st.o[t][dt], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int dt = 0; dt < 4; dt++)
+              st.o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][dt]), p[j],
+                                                                 st.o[t][dt], 0, 0, 0);
+        }
+      }
+    };
+
+    for (int base = s0; base < hi; base += step) {
+      const int32_t sc = base + (lane & (SB - 1)) < hi ? spl : -1;
+      scores();
+      // (loaded past the last batch too, from the last slot: a branch around the
+      // loads would have the next wait drain them all)
+      load_k(base + step);
+      const uint64_t all = __ballot((sc >= 0) & (sc < p0) & (p0 + deepest - sc < a.C));
+      if (~all) {  // uniform
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const int32_t at = p0 + __popcll(masks_of(anc, t)) - 1;
+#pragma unroll
+          for (int j = 0; j < NS; j++) {
+            const int32_t p = __shfl(sc, 16 * (j >> 2) + 4 * g + (j & 3));
+            s[t][j] = ((p >= 0) & (p < p0) & (at - p < a.C)) ? s[t][j] : -INFINITY;
+          }
+        }
+      }
+      apply();
+      load_v(base + step);
+    }
+    uint64_t kept = anc;
+    if (deepest >= a.C) {  // uniform: chains longer than the ring lose their first nodes, as appended rows do
+      const int depth = __popcll(anc);
+      for (int i = 0; i < n; i++)
+        if (depth - __builtin_amdgcn_readlane(depth, i) >= a.C) kept &= ~(1ull << i);
+    }
     for (int base = wave * SB; base < keys; base += kTreeWaves * SB) {
       if constexpr (KV_BF16) {
 #pragma unroll
@@ -663,7 +669,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
       scores();
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const uint64_t sees = ancestors_of(t);
+        const uint64_t sees = masks_of(kept, t);
 #pragma unroll
         for (int j = 0; j < NS; j++) {
           const int row = base + 16 * (j >> 2) + 4 * g + (j & 3);
@@ -672,60 +678,59 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
       }
       apply();
     }
-  }
 
-  // join the waves' states, a tile of 16 nodes at a time
-  bool bad = false;
+    // join the waves' states, a tile of 16 nodes at a time
+    bool bad = false;
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const float l = col_sum(st.l[t]);
-    __syncthreads();
-    float* f = sq + (wave * 16 + c) * PART;
+    for (int t = 0; t < NT; t++) {
+      const float l = col_sum(st.l[t]);
+      __syncthreads();
+      float* f = sq + (wave * 16 + c) * PART;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      *(f32x4_t*)(f + 16 * g + 4 * i) = f32x4_t{st.o[t][0][i], st.o[t][1][i], st.o[t][2][i], st.o[t][3][i]};
-    if (g == 0) {
-      f[64] = st.m[t];
-      f[65] = l;
-    }
-    __syncthreads();
-    const int i = tid >> 4, d = (tid & 15) * 4, node = node0 + 16 * t + i;
-    float M = -INFINITY, L = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 4; i++)
+        *(f32x4_t*)(f + 16 * g + 4 * i) = f32x4_t{st.o[t][0][i], st.o[t][1][i], st.o[t][2][i], st.o[t][3][i]};
+      if (g == 0) {
+        f[64] = st.m[t];
+        f[65] = l;
+      }
+      __syncthreads();
+      const int i = tid >> 4, d = (tid & 15) * 4, node = node0 + 16 * t + i;
+      float M = -INFINITY, L = 0.f;
+      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; w++) M = fmaxf(M, sq[(w * 16 + i) * PART + 64]);
+      for (int w = 0; w < kTreeWaves; w++) M = fmaxf(M, sq[(w * 16 + i) * PART + 64]);
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; w++) {
-      const float* r = sq + (w * 16 + i) * PART;
-      const float by = M == -INFINITY ? 0.f : __expf(r[64] - M);
-      L += by * r[65];
-      o += by * *(const f32x4_t*)(r + d);
-    }
-    if (node < n) {
-      bad |= !(fabsf(o[0]) < INFINITY && fabsf(o[1]) < INFINITY && fabsf(o[2]) < INFINITY &&
-               fabsf(o[3]) < INFINITY && fabsf(L) < INFINITY && M < INFINITY);
-      if (part) {
-        float* pp = part + (node - node0) * PART;
-        *(f32x4_t*)(pp + d) = o;
-        if (d == 0) {
-          pp[64] = M;
-          pp[65] = L;
+      for (int w = 0; w < kTreeWaves; w++) {
+        const float* r = sq + (w * 16 + i) * PART;
+        const float by = M == -INFINITY ? 0.f : __expf(r[64] - M);
+        L += by * r[65];
+        o += by * *(const f32x4_t*)(r + d);
+      }
+      if (node < n) {
+        bad |= !(fabsf(o[0]) < INFINITY && fabsf(o[1]) < INFINITY && fabsf(o[2]) < INFINITY &&
+                 fabsf(o[3]) < INFINITY && fabsf(L) < INFINITY && M < INFINITY);
+        if (part) {
+          float* pp = part + (node - node0) * PART;
+          *(f32x4_t*)(pp + d) = o;
+          if (d == 0) {
+            pp[64] = M;
+            pp[65] = L;
+          }
+        } else {
+          float* op = a.out + ((int64_t)b * a.rows + node) * a.out_stride + head * HD + d;
+          const float by = L == 0.f ? 0.f : 1.f / L;
+          *(f32x4_t*)op = o * by;
         }
-      } else {
-        float* op = a.out + ((int64_t)b * a.rows + node) * a.out_stride + head * HD + d;
-        const float by = L == 0.f ? 0.f : 1.f / L;
-        *(f32x4_t*)op = o * by;
       }
     }
-  }
-  const bool any = __ballot(bad) != 0;
-  if (lane == 0) flag[wave] = any;
-  __syncthreads();
-  static_assert(kTreeWaves == 4, "four flags");
-  if (flag[0] | flag[1] | flag[2] | flag[3]) {
-    exact_rows<KV_BF16>(a, tid, b, head, lo, hi, drafts, part, node0, min(n, node0 + NN), p0, anc, sdk, sdv, DP);
+    const bool any = __ballot(bad) != 0;
+    if (lane == 0) flag[wave] = any;
     __syncthreads();
-  }
+    static_assert(kTreeWaves == 4, "four flags");
+    if (flag[0] | flag[1] | flag[2] | flag[3]) {
+      exact_rows<KV_BF16>(a, tid, b, head, lo, hi, drafts, part, node0, min(n, node0 + NN), p0, anc, sdk, sdv, DP);
+      __syncthreads();
+    }
   }
 }
 

@@ -59,6 +59,7 @@ def tree_reference(ring, qkv, parent, pos0, n, bf16):
     out, bound = np.zeros((n, D)), np.zeros((n, D))
     for i, c in enumerate(cs):
         pos = pos0 + len(c) - 1
+        c = c[-C:]  # those that its window holds
         live = (sp >= 0) & (sp < pos0) & (pos - sp.astype(np.int64) < C)
         kk = np.concatenate((k[live], ks[c])).astype(np.float64).reshape(-1, H, HD)
         vv = np.concatenate((v[live], vs[c])).astype(np.float64).reshape(-1, H, HD)

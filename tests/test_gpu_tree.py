@@ -157,6 +157,31 @@ def test_tree_equals_appending_its_paths(name, kv):
 
 
 @pytest.mark.parametrize("name,kv", KV)
+@pytest.mark.parametrize("bad", [False, True])
+@pytest.mark.parametrize("T,C,pos0", [(2, 1, 0), (2, 1, 7), (20, 3, 0), (40, 33, 50), (64, 7, 2), (64, 63, 200)])
+def test_tree_of_chains_longer_than_the_ring(name, kv, bad, T, C, pos0):
+    """A node does not see ancestors that its own appends would have evicted: the
+    result is that of appending the chain row by row."""
+    say(f"long chains T={T} C={C} pos0={pos0} kv={name} bad={bad}")
+    rng = np.random.default_rng([T, C, pos0, bad])
+    parent = np.stack((np.arange(-1, T - 1), np.maximum(np.arange(T) - 2, -1))).astype(np.int32)
+    at, n = np.full(2, pos0, np.int32), np.full(2, T, np.int32)
+    qkv = rng.standard_normal((2, T, QKV), dtype=np.float32)
+    if bad:  # evicted by the last row of the first chain, and seen by earlier ones
+        qkv[0, 0, 2 * D] = np.inf
+    with mb.Context(n_layers=1, capacity=C, max_seqs=2, max_rows=64, kv_dtype=kv) as ctx:
+        _fill(ctx, rng, 0, at)
+        got = ctx.tree_attention(0, qkv, parent, at, n)
+        for b in range(2):
+            want, bound = tree_reference(ctx.read_ring(0, b), qkv[b], parent[b], pos0, T, kv == mb.MB_KV_BF16)
+            fine = np.isfinite(want)
+            assert np.array_equal(got[b][~fine], want[~fine].astype(np.float32), equal_nan=True)
+            assert (np.abs(got[b] - want)[fine] <= bound[fine]).all()
+            assert fine.all() == (b == 1 or not bad)
+            assert fine[-1].all()
+
+
+@pytest.mark.parametrize("name,kv", KV)
 def test_tree_does_not_see_a_dropped_draft(name, kv):
     """Slots at pos0 and later (an earlier draft, rolled back) are not seen, in
     whatever state."""
