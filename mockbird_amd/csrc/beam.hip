@@ -270,7 +270,7 @@ __device__ __forceinline__ void scan_row(const void* row, const uint32_t* seen, 
         for (int e = 0; e < PER; e++) {
           // (the double product rounds once to the fp32 product, and with the
           // reciprocal to the fp32 quotient: no quotient of two floats is
-          // within 2^-50 of the middle between two floats)
+          // within 2^-50 of the middle between two normal floats)
           float& x = z[q * PER + e];
           const float y = (float)((double)x * (x < 0.f ? (double)penalty : by));
           x = (bits >> e) & 1 ? y : x;

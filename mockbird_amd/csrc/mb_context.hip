@@ -248,16 +248,22 @@ int check_beam(mb_ctx* ctx, int B, int width, int vocab, int n_out) {
   return MB_OK;
 }
 
-int check_beam_options(mb_ctx* ctx, int vocab, const void* scores, const void* done, int32_t end_id,
-                       const void* seen, double penalty, const void* scores_out,
-                       const void* done_out, const void* seen_out) {
+bool overlap(const void* a, int64_t an, const void* b, int64_t bn) {
+  return a && b && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
+int check_beam_options(mb_ctx* ctx, int B, int width, int vocab, int n_out, const void* scores,
+                       const void* done, int32_t end_id, const void* seen, double penalty,
+                       const void* scores_out, const void* done_out, const void* seen_out) {
   if (end_id < -1 || end_id >= vocab || (done && end_id < 0))
     return fail(ctx, MB_ERR_ARG, "end_id %d is no id of %d (-1 where no beam is done)", end_id, vocab);
   if (seen_out && !seen) return fail(ctx, MB_ERR_ARG, "seen_out needs seen");
-  if (seen && (!(penalty > 0.0) || !(penalty < INFINITY)))
-    return fail(ctx, MB_ERR_ARG, "penalty %g is not a positive number", penalty);
-  if ((scores && scores == scores_out) || (done && done == done_out) || (seen && seen == seen_out))
-    return fail(ctx, MB_ERR_ARG, "an output is its input");
+  if (seen && (!((float)penalty > 0.f) || !((float)penalty < INFINITY)))
+    return fail(ctx, MB_ERR_ARG, "penalty %g is not a positive fp32 number", penalty);
+  const int64_t rows = (int64_t)B * width * 4, outs = (int64_t)B * n_out * 4, words = ((int64_t)vocab + 31) / 32;
+  if (overlap(scores, rows, scores_out, outs) || overlap(done, rows, done_out, outs) ||
+      overlap(seen, rows * words, seen_out, outs * words))
+    return fail(ctx, MB_ERR_ARG, "an output overlaps its input");
   return MB_OK;
 }
 
@@ -704,6 +710,14 @@ int mb_tree_attention_dev(mb_ctx* ctx, int layer, int B, int rows_max, const voi
     return fail(ctx, MB_ERR_ARG, "rows must start at multiples of 16 bytes");
   rc = check_work(ctx, work, work_bytes, tree_work_bytes(ctx, B, rows_max, max_pos));
   if (rc) return rc;
+  const int64_t n = (int64_t)B * rows_max - 1, in = qkv_stride * (qkv_dtype == MB_DT_BF16 ? 2 : 4),
+                row = QKV * (qkv_dtype == MB_DT_BF16 ? 2 : 4);
+  if (overlap(qkv, n * in + row, out, (n * out_stride + D) * 4)) {
+    // rows that lie between one another are right
+    const int64_t at = (((intptr_t)out - (intptr_t)qkv) % in + in) % in;
+    if (in != out_stride * 4 || at < row || at + D * 4 > in)
+      return fail(ctx, MB_ERR_ARG, "out overlaps qkv");
+  }
   return launch_tree_attention(ctx, global_ring(ctx, layer), B, rows_max, qkv, qkv_dtype, qkv_stride,
                                parent, pos0, n_nodes, max_pos, out, out_stride, work);
 }
@@ -749,7 +763,8 @@ int mb_beam_select_dev(mb_ctx* ctx, int B, int width, int vocab, int n_out, cons
   if (logits_dtype != MB_DT_F32 && logits_dtype != MB_DT_BF16)
     return fail(ctx, MB_ERR_ARG, "unknown dtype");
   if (logits_stride < vocab) return fail(ctx, MB_ERR_ARG, "row stride too small");
-  rc = check_beam_options(ctx, vocab, scores, done, end_id, seen, penalty, scores_out, done_out, seen_out);
+  rc = check_beam_options(ctx, B, width, vocab, n_out, scores, done, end_id, seen, penalty, scores_out,
+                          done_out, seen_out);
   if (rc) return rc;
   if (B == 0) return MB_OK;
   if (!logits || !scores || !scores_out || !parent || !token)
@@ -1045,7 +1060,8 @@ int mb_beam_select(mb_ctx* ctx, int B, int width, int vocab, int n_out, const fl
   MB_DEVICE_GUARD(ctx);
   int rc = check_beam(ctx, B, width, vocab, n_out);
   if (rc) return rc;
-  rc = check_beam_options(ctx, vocab, scores, done, end_id, seen, penalty, scores_out, done_out, seen_out);
+  rc = check_beam_options(ctx, B, width, vocab, n_out, scores, done, end_id, seen, penalty, scores_out,
+                          done_out, seen_out);
   if (rc) return rc;
   if (B == 0) return MB_OK;
   if (!logits || !scores || !scores_out || !parent || !token)

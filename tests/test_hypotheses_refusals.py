@@ -81,6 +81,9 @@ def tree_dev(h, layer=0, B=1, rows=8, qkv=P, dtype=0, stride=2304, parent=P, pos
     (dict(dtype=1, stride=2308), "16 bytes"), (dict(out_stride=770), "16 bytes"), (dict(out=P + 4), "16 bytes"),
     (dict(max_pos=5000, work=None), "workspace"), (dict(max_pos=5000, work_bytes=100), "workspace"),
     (dict(max_pos=5000, work=P + 8), "workspace"),
+    (dict(), "out overlaps"), (dict(out=P + 8 * 2304 * 4 - 16), "out overlaps"),
+    (dict(stride=3084, out_stride=3084, out=P + 2304 * 4 - 16), "out overlaps"),
+    (dict(stride=3068, out_stride=3068, out=P + 2304 * 4), "out overlaps"),
 ])
 def test_tree_attention_dev_refuses(bare, kw, words):
     _refused(h := bare(capacity=5000), tree_dev(h, **kw), mb.MB_ERR_ARG, words)
@@ -166,7 +169,7 @@ def test_tree_commit_refuses(bare, change, words, code):
     _refused(h, rc, code, words)
 
 
-Q = P << 1
+Q = 1 << 40
 
 
 def beam_dev(h, B=2, W=4, V=100, n=4, logits=P, dtype=0, stride=100, scores=P, done=P, end=7, seen=P,
@@ -185,12 +188,14 @@ def beam_dev(h, B=2, W=4, V=100, n=4, logits=P, dtype=0, stride=100, scores=P, d
     (dict(penalty=0.0), "penalty"), (dict(penalty=-1.0), "penalty"),
     (dict(penalty=float("nan")), "penalty"), (dict(penalty=float("inf")), "penalty"),
     (dict(scores_out=P), "its input"), (dict(done_out=P), "its input"), (dict(seen_out=P), "its input"),
+    (dict(scores_out=P + 28), "its input"), (dict(done=Q + 28), "its input"), (dict(seen=Q + 124), "its input"),
+    (dict(penalty=1e-60), "penalty"), (dict(penalty=1e300), "penalty"),
     (dict(logits=None), "null"), (dict(scores=None), "null"), (dict(scores_out=None), "null"),
     (dict(parent=None), "null"), (dict(token=None), "null"),
     (dict(V=5000, stride=5000, work=None), "workspace"),
     (dict(V=5000, stride=5000, work_bytes=64), "workspace"),
     (dict(V=5000, stride=5000, work=P + 8), "workspace"),
-    (dict(B=2 ** 31 - 1), "too many rows"),
+    (dict(B=2 ** 31 - 1, scores_out=1 << 60, done_out=1 << 60, seen_out=1 << 60), "too many rows"),
 ])
 def test_beam_select_dev_refuses(bare, kw, words):
     h = bare()
