@@ -41,6 +41,7 @@ struct TreeIn {
   float* out;
   int64_t out_stride;
   int B, pieces;  // pieces 0: a workgroup per (sequence, head, group)
+  int cus;        // then, if not 0: those in the order of their work, this many at a time
   int32_t* plan;  // kPlanWords: the sequences' places on the line, and a piece's length
   float* part;    // two states per workgroup and row
 };
@@ -58,10 +59,8 @@ __device__ __forceinline__ int tree_size(const int32_t* pos0, const int32_t* n_n
 // sequences' quanta follow one another, and the line is cut into `pieces` equal
 // ones, one for each workgroup of a head (and group of nodes).  So all
 // workgroups have the same work whatever the windows' lengths are, and all fit
-// the chip at once.  (A workgroup for each sequence and head, or for each equal
-// share of a window, ended at 35 to 66 us over 24 windows of up to 1001 slots; more
-// and smaller workgroups than fit at once start under load, where each of their
-// three trips to memory takes several us.)
+// the chip at once.  (More and smaller workgroups than fit at once start under
+// load, where each of their three trips to memory takes several us.)
 // A state of a sequence that was cut goes to place 0 of its workgroup where the
 // sequence began before the piece, else to place 1.
 constexpr int kLineSeqs = 64, kPlanWords = 192;  // sequences on a line; words of TreeIn::plan
@@ -100,6 +99,55 @@ __device__ __forceinline__ int lay_line(const TreeIn& a, int piece, int lane, bo
   const uint64_t who = __ballot(at >= upto - q && at < upto);
   first = who ? __ffsll((unsigned long long)who) - 1 : 0;
   return total;
+}
+// Workgroups for each (sequence, head, group) in the order of their work.  Such a
+// launch fits the chip at once, its workgroups i, i + cus, i + 2 cus .. on one CU, so
+// the time is that of the CU with the most work (24 voices of 17 to 61 nodes over up
+// to 1001 fp32 slots: 57.5 us in the sequences' order, 46.5 in this).  The longest come first and every
+// second round of cus runs backwards, which puts short ones to the longest.
+// Returns the sequence of this workgroup (-1: none), and its head and group; all
+// waves count ranks, 16 sequences each.
+template <int QS, int NT, int G>
+__device__ __forceinline__ int by_work(const TreeIn& a, int lane, int wave, int32_t* ranks,
+                                       int& head, int& group, int& p0_of, int& n_of) {
+  int p0 = 0, n = 0;
+  if (lane < a.B) n = tree_size(a.pos0, a.n_nodes, a.rows, lane, p0);
+  uint32_t key[G];  // the work, and the lower sequence of the first group first
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    const int tiles = min(NT, (n - g * 16 * NT + 15) >> 4);
+    key[g] = tiles > 0 ? (uint32_t)(tiles * (1 + (min(p0, a.C) + QS - 1) / QS)) << 7 | (127 - 64 * g - lane) : 0u;
+  }
+  int above[G] = {};
+  const int j0 = wave * (kLineSeqs / kTreeWaves), j1 = min(a.B, j0 + kLineSeqs / kTreeWaves);
+  for (int j = j0; j < j1; j++)
+#pragma unroll
+    for (int h = 0; h < G; h++) {
+      const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)key[h], j);
+#pragma unroll
+      for (int g = 0; g < G; g++) above[g] += other > key[g];
+    }
+#pragma unroll
+  for (int g = 0; g < G; g++) ranks[(wave * G + g) * 64 + lane] = above[g];
+  __syncthreads();
+  const int round = blockIdx.x / a.cus, at = blockIdx.x - round * a.cus;
+  const int i = round * a.cus + (round & 1 ? a.cus - 1 - at : at), rank = i / H;
+  head = i - rank * H;
+  int b = -1;
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    int r = 0;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; w++) r += ranks[(w * G + g) * 64 + lane];
+    const uint64_t who = __ballot(key[g] != 0u && r == rank);
+    if (who) {
+      b = __ffsll((unsigned long long)who) - 1;
+      group = g;
+    }
+  }
+  p0_of = __builtin_amdgcn_readlane(p0, max(b, 0));
+  n_of = __builtin_amdgcn_readlane(n, max(b, 0));
+  return b;
 }
 // A workgroup's states of its place 0 or 1.
 __device__ __forceinline__ float* states(const TreeIn& a, int share, int group, int groups, int rows, int place) {
@@ -324,12 +372,13 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
   // first group, which has the more nodes, fell to every other CU.)
   constexpr int QS = kTreeWaves * SB;
   const int shares = G == 1 ? gridDim.x : gridDim.x / G;
-  const int group = G == 1 ? 0 : blockIdx.x / shares, share = blockIdx.x - group * shares;
-  const int piece = share / H, head = share % H;
-  const int node0 = group * NN;  // this group's first node
+  int group = G == 1 ? 0 : blockIdx.x / shares;
+  const int share = blockIdx.x - group * shares, piece = share / H;
+  int head = share % H;
   __shared__ Line line;
   __shared__ int32_t flag[kTreeWaves];
   int first = piece, end = a.B, from = 0, to = 0;  // the piece: quanta [from, to) from sequence `first` on
+  int one_p0 = 0, one_n = 0;
   if (a.pieces) {
     if (G > 1 && piece >= a.pieces) return;
     int length;
@@ -344,9 +393,18 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
     to = min(total, from + length);
     if (from >= to) return;
   } else {
-    if (G > 1 && piece >= a.B) return;
-    end = piece + 1;
+    if (a.cus) {
+      // (the counts where q's rows will be)
+      static_assert(kTreeWaves * G * 64 <= NN * QP, "the angles are written while others read them");
+      first = by_work<QS, NT, G>(a, lane, wave, (int32_t*)sq, head, group, one_p0, one_n);
+      if (first < 0) return;
+    } else {
+      if (G > 1 && piece >= a.B) return;
+      one_n = tree_size(a.pos0, a.n_nodes, a.rows, first, one_p0);
+    }
+    end = first + 1;
   }
+  const int node0 = group * NN;  // this group's first node
 
   for (int b = first; b < end; b++) {
     // (the thread's places are worked out anew for each sequence: kept over the
@@ -359,7 +417,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
       p0 = line.p0[b];
       n = line.n[b];
     } else {
-      n = tree_size(a.pos0, a.n_nodes, a.rows, b, p0);
+      p0 = one_p0;
+      n = one_n;
     }
     p0 = __builtin_amdgcn_readfirstlane(p0);
     n = __builtin_amdgcn_readfirstlane(n);
@@ -794,21 +853,25 @@ __global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a, int groups) 
 // and heads two per CU.  (us for 24 voices of up to 61 nodes in fp32 / 3 of 64 over
 // 16384 slots / 8 of 16 over 2048, bf16: one per CU 57.2 / 55.4 / 17.3, two 57.1 /
 // 48.0 / 17.8, three, as many as fit, 61.1 / 49.3 / 18.2.)  0: a workgroup for each
-// sequence, where a piece would not be shorter than the longest window by
-// kLineGain quanta, which is what the second launch and the sequences that begin
-// inside a piece cost.  (us as sequences / as a line, by voices x nodes x slots of
-// full quanta: 1 x 8 x 1024 fp32 17.5 / 9.4, 4 x 32 x 512 fp32 17.0 / 12.8, 8 x 16 x 2048
-// bf16 20.2 / 19.1, 10 x 2 x 1139 bf16 14.0 / 15.6, 16 x 16 x 1024 bf16 13.8 / 19.2, 30 x 16
-// x 1000 bf16 21.7 / 25.7, 12 x 48 x 700 bf16 17.1 / 25.0, 64 x 16 x 2048 bf16 61 / 75.)
-constexpr int kLineGain = 6;
+// sequence, where a piece is not shorter than the longest window by what the line
+// costs: kLineGain quanta for the second launch and the sequences that begin
+// inside a piece, and up to kLineShare for two pieces on a CU that has one
+// sequence.  (us as a line / as sequences, by voices x nodes x slots: 1 x 8 x 1024 fp32
+// 9.4 / 17.5, 4 x 32 x 512 fp32 12.4 / 16.9, 8 x 16 x 2048 bf16 18.8 / 20.4, 12 x 16 x 4000
+// bf16 31.7 / 40.0, 28 x 16 x 8000 bf16 103 / 119, 10 x 64 x 4096 fp32 87 / 92; 10 x 2 x
+// 1139 bf16 15.6 / 14.0, 16 x 16 x 1024 bf16 19.1 / 13.9, 24 x 30 x 1001 fp32 41.3 / 36.9,
+// 12 x 64 x 2000 bf16 34.9 / 30.2, 21 x 64 x 1001 fp32 62.7 / 54.6; 24 x 8 x 4096 fp32, 86.5
+// / 83.6, is taken as a line.)
+constexpr int kLineGain = 5, kLineShare = 15;
+static int tree_cus(const mb_ctx* ctx) { return ctx->cus_per_xcd > 0 ? ctx->xcds * ctx->cus_per_xcd : 256; }
 static int tree_groups(int rows) { return rows <= 32 ? 1 : 2; }
 static int tree_pieces(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
-  const int cus = ctx->cus_per_xcd > 0 ? ctx->xcds * ctx->cus_per_xcd : 256;
+  const int cus = tree_cus(ctx);
   const int pieces = std::max(1, 2 * cus / (H * tree_groups(rows)));
   const int qs = kTreeWaves * (ctx->cfg.kv_dtype == MB_KV_BF16 ? 32 : 16);
   const int window = (std::min(max_pos, ctx->cfg.capacity) + qs - 1) / qs;
   const int piece = (int)(((int64_t)B * (1 + window) + pieces - 1) / pieces);
-  return B <= kLineSeqs && window - piece >= kLineGain ? pieces : 0;
+  return B <= kLineSeqs && window - piece >= kLineGain + std::min(piece, kLineShare) ? pieces : 0;
 }
 
 int64_t tree_work_bytes(const mb_ctx* ctx, int B, int rows, int32_t max_pos) {
@@ -842,10 +905,12 @@ int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, co
   a.plan = (int32_t*)work;
   a.part = (float*)work + kPlanWords;
   const int groups = tree_groups(rows);
+  const int cus = tree_cus(ctx);
+  a.cus = a.pieces == 0 && B <= kLineSeqs && B * H * groups > cus ? cus : 0;
   const unsigned shares = (unsigned)((a.pieces ? a.pieces : B) * H);
   auto go = [&](auto nt, auto g) {
     constexpr int NT = decltype(nt)::value, G = decltype(g)::value;
-    const dim3 grid(G == 1 ? shares : (shares + 7) / 8 * 8 * G);
+    const dim3 grid(a.cus ? (shares * G + a.cus - 1) / a.cus * a.cus : G == 1 ? shares : (shares + 7) / 8 * 8 * G);
     if (ring.bf16) hipLaunchKernelGGL((k_tree<true, NT, G>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
     else hipLaunchKernelGGL((k_tree<false, NT, G>), grid, dim3(64 * kTreeWaves), 0, ctx->stream, a);
   };

@@ -79,7 +79,7 @@ def test_tree_attention_split_and_many(name, kv, B, T, C):
 
 
 @pytest.mark.parametrize("name,kv", KV)
-@pytest.mark.parametrize("B,T", [(20, 40), (21, 33), (22, 64), (41, 17), (42, 16), (43, 5), (65, 2)])
+@pytest.mark.parametrize("B,T", [(20, 40), (21, 33), (22, 64), (41, 17), (42, 16), (43, 5), (64, 50), (64, 3), (65, 2)])
 def test_tree_attention_as_sequences_and_as_a_line(name, kv, B, T):
     """Around the numbers of sequences from which each has workgroups of its own;
     windows of all lengths, several sequences without nodes or rows."""
