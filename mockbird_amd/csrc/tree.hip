@@ -234,10 +234,9 @@ __device__ __forceinline__ void rope8(const float2 (&t)[4], float* x) {
   }
 }
 
-// Part of a ring row, with the streaming hint where the launch reads it once.
-template <bool ONCE, class T>
-__device__ __forceinline__ T ring_load(const char* p) {
-  return ONCE ? __builtin_nontemporal_load((const T*)p) : *(const T*)p;
+// The first `bytes` bytes from p on, as a buffer whose loads past the end give zeros.
+__device__ __forceinline__ auto buffer_of(const char* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00027000);
 }
 
 // One element of a K or V row.
@@ -473,30 +472,26 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
 
     TreeBatch<KV_BF16> x;
     int32_t spl;  // lane l: the stored position of the batch's slot l % SB
-    // Slots past the window read its last one (slot 0 of an empty window) and
-    // are dead by their position.  (A head's run is at most 2^28 bytes.)
-    const int last = max(hi - 1, 0);
+    // Slots from hi on are past the buffers' ends: they load as zeros and are dead by
+    // their number.  (A head's run is at most 2^28 bytes.)
+    const auto kr = buffer_of(kb, hi * ROWB), vr = buffer_of(vb, hi * ROWB), pr = buffer_of((const char*)sp, hi * 4);
+    constexpr int ONCE = G == 1 ? 2 : 0;  // the streaming hint where the launch reads a row once
     auto load_k = [&](int base) {
-      spl = sp[min(base + (lane & (SB - 1)), last)];
-      if constexpr (KV_BF16) {
+      spl = (int32_t)__builtin_amdgcn_raw_buffer_load_b32(pr, (base + (lane & (SB - 1))) * 4, 0, 0);
+      const int at = base * ROWB + c * ROWB + g * 16;
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const char* r = kb + (uint32_t)(min(base + 16 * u + c, last) * ROWB + g * 16);
-#pragma unroll
-          for (int h = 0; h < 2; h++) x.k[2 * u + h] = ring_load<G == 1, u32x4_t>(r + 64 * h);
-        }
-      } else {
-        const char* r = kb + (uint32_t)(min(base + c, last) * ROWB + g * 16);
-#pragma unroll
-        for (int q = 0; q < 4; q++) x.k[q] = ring_load<G == 1, u32x4_t>(r + 64 * q);
-      }
+      for (int i = 0; i < 4; i++)
+        x.k[i] = __builtin_bit_cast(
+            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                         kr, at + (KV_BF16 ? 16 * ROWB * (i >> 1) + 64 * (i & 1) : 64 * i), 0, ONCE));
     };
     auto load_v = [&](int base) {
+      const int at = base * ROWB + 4 * g * ROWB + c * 4 * E;
 #pragma unroll
       for (int j = 0; j < NS; j++) {
-        const char* r = vb + (uint32_t)(min(base + 16 * (j >> 2) + 4 * g + (j & 3), last) * ROWB + c * 4 * E);
-        if constexpr (KV_BF16) x.v[j] = ring_load<G == 1, u32x2_t>(r);
-        else x.v[j] = ring_load<G == 1, u32x4_t>(r);
+        const int row = at + (16 * (j >> 2) + (j & 3)) * ROWB;
+        if constexpr (KV_BF16) x.v[j] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(vr, row, 0, ONCE));
+        else x.v[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, row, 0, ONCE));
       }
     };
     const int s0 = lo + wave * SB, step = kTreeWaves * SB;
