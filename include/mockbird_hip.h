@@ -319,7 +319,7 @@ int mb_tree_commit_dev(mb_ctx* ctx, int layer0, int n_layers, int B, int rows_ma
  * logit is multiplied by the penalty when negative and divided when not, in
  * fp32 with the penalty rounded to fp32 (MB_PENALTY_F32's arithmetic).  A beam
  * with done[b][w] != 0 goes on as it is: its one continuation is end_id with
- * c = scores[b][w] (its logits are not read).  c is formed and compared in
+ * c = scores[b][w], whatever its logits are.  c is formed and compared in
  * double; ties go to the lower beam, then the higher logit, then the lower id.
  * A NaN or -inf logit is never chosen, nor a beam whose score is NaN or -inf;
  * +inf logits share the whole probability.  For k < n_out, best first:

@@ -69,7 +69,7 @@ __device__ __forceinline__ uint64_t order_of(double c) {
 // Raises lo, which at_lo >= n of some keys reach, until hardly more than n do, by
 // the counts of keys that reach WAYS - 1 bounds between lo and hi (which no key
 // exceeds).  count(bound) is uniform.  (A step is a chain of compare, count and
-// branch of some 300 cycles whatever WAYS is: by halves 8 steps took 2400.)
+// branch of some 300 cycles whatever WAYS is, so few steps of many bounds.)
 constexpr int kSlack = 8;
 template <int WAYS, class Count>
 __device__ __forceinline__ void raise(uint32_t& lo, int& at_lo, uint32_t hi, int n, Count count) {
@@ -352,7 +352,11 @@ __device__ __forceinline__ void part_empty(const BeamIn& a, int64_t row, int chu
   if (lane < a.n) ((uint2*)(p + sizeof(PartRow)))[lane] = make_uint2(__float_as_uint(-INFINITY), kNoId);
 }
 
-// A wave per part of a row.
+// A wave per part of a row.  16 voices x 8 beams x 32000 fp32 ids, 16 chosen (16.4 MB): 9.1
+// us, where reading them takes 2.4: four waves a SIMD, each one part, whose
+// exponentials, bound and list are some 4000 cycles of vector instructions in
+// one chain (with n rounds of the wave's best instead of the bound and the ranks,
+// here and in the choice, the two launches took 56 us, not 19).
 __global__ __launch_bounds__(256) void k_beam_scan(const BeamIn a, int64_t parts) {
   __shared__ __align__(16) uint64_t buf[4][66];
   const int lane = threadIdx.x & 63;
@@ -478,6 +482,10 @@ __device__ __forceinline__ int best_of(uint64_t* lk, int all, int n, int lane, u
 // One workgroup per voice, its waves taking the beams' rows in turn; then the
 // first wave takes the n best of the W n candidates by c.  On equal c the lower
 // beam goes first and, within a beam, the list's order holds.
+// A chain that one workgroup a voice walks: 1 voice x 4 beams x 1024 ids 6.1 us, 64 x 8 x
+// 1024 with a penalty 9.4 (2 MB of logits), the join of 16 x 8 rows in 32 parts of 16
+// ids 11.3; the ranks by counting instead of rounds took 9.2 us to 5.3 and 17.5 to 8.6,
+// calls of the first two.
 constexpr int kBeamWaves = 16;
 template <bool FUSED>
 __global__ __launch_bounds__(64 * kBeamWaves) void k_beam_pick(const BeamIn a) {
@@ -689,6 +697,8 @@ struct ReorderIn {
 // group: it reads the parents' before it writes any, so the move is in place
 // and every byte is read where its parent still has it.  A group's slots are
 // cut into blockDim.x-thread pieces along blockIdx.y.
+// 32 voices x 4 beams x 12 layers, 300 bf16 rows each (1.5 GB read and written): 290
+// us, 5.2 TB/s, where a copy of 2 GiB reaches 4.87.
 template <int MW>
 __global__ __launch_bounds__(256) void k_ring_reorder(const ReorderIn a, int chunk_bits) {
   const int head = blockIdx.x % H;

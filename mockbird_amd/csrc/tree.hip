@@ -245,11 +245,22 @@ __device__ __forceinline__ float elem(const char* row, int d) {
   return BF16 ? bf16_lo(((const uint16_t*)row)[d]) : ((const float*)row)[d];
 }
 
-// One workgroup per head and piece of the line (or sequence).  A wave takes batches of SB slots
-// (8 KB of K and V) in turn with the other waves of its (sequence, head),
-// forms the scores of all nodes, 16 to a tile, and keeps its own softmax state
-// per node; the waves' states are joined in LDS at the end, and those of
-// several workgroups by k_tree_merge.
+// One workgroup per head and sequence, or piece of the line, and group of nodes (all
+// up to 32 rows, 32 each beyond).  A wave takes batches of SB slots (8 KB of K and V)
+// in turn with the other waves of its (sequence, head), forms the scores of all
+// nodes, 16 to a tile, and keeps its own softmax state per node; the waves' states
+// are joined in LDS at the end, and those of several workgroups by k_tree_merge.
+// (With all 64 nodes' states a wave runs alone on its SIMD: 24 voices of up to 61 nodes
+// over 1001 fp32 slots 97 us; groups of 32, three waves to a SIMD, and the rope
+// table's rows read at once, 72.)
+//
+// What bounds it, by the kernel's own time: 64 voices x 16 nodes over up to 2048 bf16
+// slots, 62 us: HBM, 335 MB at 5.4 TB/s.  24 x 17 .. 61 over up to 1001 fp32 slots, 44
+// us: the fp32 matrix instructions, 18.7 us a SIMD on average and a quarter more
+// on the CU with the most, between the starts and the joins.  3 x 40 .. 64 over up to
+// 16384 bf16 slots, 45 us: two waves a SIMD take 19 us of vector instructions (the
+// exponentials and the planes of the weights) and 9 of matrix ones, in one chain
+// a wave.  1 x 8 over 1024 fp32 slots, 5.6 us: three trips to memory.
 //
 // Scores are formed as S^T = K Q^T, 16 slots x 16 nodes: lane (c = lane % 16,
 // g = lane / 16) of the accumulator holds slots 4g .. 4g + 3 of node c, which is
@@ -490,8 +501,10 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
 #pragma unroll
       for (int j = 0; j < NS; j++) {
         const int row = at + (16 * (j >> 2) + (j & 3)) * ROWB;
-        if constexpr (KV_BF16) x.v[j] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(vr, row, 0, ONCE));
-        else x.v[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, row, 0, ONCE));
+        if constexpr (KV_BF16)
+          x.v[j] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(vr, row, 0, ONCE));
+        else
+          x.v[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, row, 0, ONCE));
       }
     };
     const int s0 = lo + wave * SB, step = kTreeWaves * SB;
@@ -790,7 +803,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, 3) void k_tree(const TreeIn a) {
 
 // The states of a sequence that was cut: a wave per node of one (sequence,
 // head), lane (g, quad) taking every fourth state's dims 4 quad .. + 3, 16 states
-// on their way at once.
+// on their way at once: two trips to memory, 4.0 us over 8 sequences of 16 nodes, 4.9
+// over 3 of 64.
 __global__ __launch_bounds__(256) void k_tree_merge(const TreeIn a, int groups) {
   const int b = blockIdx.x / H, head = blockIdx.x % H;
   const int lane = threadIdx.x & 63, g = lane >> 4, d = (lane & 15) * 4;
@@ -930,6 +944,10 @@ int launch_tree_attention(mb_ctx* ctx, const RingView& ring, int B, int rows, co
 // Each thread owns 8 dims of one head of one row of one layer; a row that a
 // later one of the same path overwrites is not stored, nor one whose node is
 // not a drafted row or whose position the ring cannot hold.
+// 64 voices x up to 8 rows x 12 layers in bf16 (21 MB): 8.0 us, 2.6 TB/s: two dependent
+// trips to memory (the path, the rows), in two rounds of waves: the rings' own cos
+// and sin of positions beyond the table, bit for bit, take 86 registers (as a
+// series, which may end a bit away, 45).  One voice: 3.4 us, a launch.
 template <bool IN_BF16, bool KV_BF16>
 __global__ __launch_bounds__(256) void k_tree_commit(
     const void* __restrict__ qkv, int64_t row_stride, int64_t layer_stride, int rows,
