@@ -96,23 +96,52 @@ def test_tree_attention_as_sequences_and_as_a_line(name, kv, B, T):
         parent = random_parents(rng, B, T)
         got = ctx.tree_attention(0, qkv, parent, pos0, n)
         _check(ctx, 0, got, qkv, parent, pos0, n, kv == mb.MB_KV_BF16)
+        # the same call again gives the same bits
+        assert np.array_equal(got, ctx.tree_attention(0, qkv, parent, pos0, n))
         n[:] = 0  # nothing at all
         out = np.full((B, T, D), 5.0, np.float32)
         assert (ctx.tree_attention(0, qkv, parent, pos0, n, out) == 5.0).all()
 
 
-@pytest.mark.parametrize("B", [3, 70])
-def test_tree_device_positions_that_do_not_fit(B):
+@pytest.mark.parametrize("name,kv", KV)
+@pytest.mark.parametrize("B,T,C", [(5, 40, 2500), (12, 3, 3000), (1, 64, 1600)])
+def test_tree_attention_of_ragged_windows_on_a_line(name, kv, B, T, C):
+    """Long windows beside short and empty ones, cut into equal pieces: sequences that
+    begin inside a piece, end in it, or have no nodes."""
+    say(f"tree line B={B} T={T} C={C} kv={name}")
+    rng = np.random.default_rng([B, T, C])
+    pos0 = rng.integers(0, 3 * C, B).astype(np.int32)
+    pos0[0], pos0[B // 2] = 2 * C + 7, 0 if B > 1 else C
+    n = rng.integers(1, T + 1, B).astype(np.int32)
+    n[0] = T
+    if B > 2:
+        n[2] = 0
+    with mb.Context(n_layers=1, capacity=C, max_seqs=B, max_rows=64, kv_dtype=kv) as ctx:
+        assert ctx.tree_attention_work(B, T, int(pos0.max())) > 0
+        _fill(ctx, rng, 0, pos0)
+        qkv = rng.standard_normal((B, T, QKV), dtype=np.float32)
+        parent = random_parents(rng, B, T)
+        out = np.full((B, T, D), 5.0, np.float32)
+        got = ctx.tree_attention(0, qkv, parent, pos0, n, out)
+        for b in range(B):
+            assert (got[b, n[b]:] == 5.0).all()
+        _check(ctx, 0, got, qkv, parent, pos0, n, kv == mb.MB_KV_BF16)
+        assert np.array_equal(got, ctx.tree_attention(0, qkv, parent, pos0, n, out.copy()))
+
+
+@pytest.mark.parametrize("B,T,C", [(3, 6, 40), (70, 6, 40), (6, 6, 1500), (6, 40, 1500), (30, 40, 40)])
+def test_tree_device_positions_that_do_not_fit(B, T, C):
     """Sequences at positions below 0 or above 2^31 - 65, and negative and too large
     counts, on the device: left out, or taken to rows_max."""
     import torch
     rng = np.random.default_rng(14)
-    T, C = 6, 40
-    pos0 = rng.integers(0, 80, B).astype(np.int32)
+    say(f"tree positions B={B} T={T} C={C}")
+    pos0 = rng.integers(0, 2 * C, B).astype(np.int32)
     n = np.full(B, T, np.int32)
     n[1] = 2 ** 31 - 1
     good = np.ones(B, bool)
-    for b, (p, m) in ((0, (-1, T)), (2, (2 ** 31 - 64, T)), (B - 2, (7, -5)), (B - 1, (-2 ** 31, T))):
+    for b, (p, m) in ((0, (-1, T)), (2, (2 ** 31 - 64, T)), (B - 2, (7, -2 ** 31 if T > 32 else -5)),
+                      (B - 1, (-2 ** 31, T))):
         pos0[b], n[b], good[b] = p, m, False
     with mb.Context(n_layers=1, capacity=C, max_seqs=B, max_rows=64) as ctx:
         _fill(ctx, rng, 0, np.where(good, pos0, 0))
@@ -202,17 +231,17 @@ def test_tree_does_not_see_a_dropped_draft(name, kv):
 
 @pytest.mark.parametrize("name,kv", KV)
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("B", [1, 70])
-def test_tree_not_finite(name, kv, bad, B):
+@pytest.mark.parametrize("B,C", [(1, 150), (24, 150), (70, 150), (1, 1500), (3, 1500)])
+def test_tree_not_finite(name, kv, bad, B, C):
     """Values that are not finite reach exactly the nodes that see them: in empty
     slots and rows behind the nodes none, in a slot that only the shallow nodes
-    still hold and in a drafted row its descendants.  (One voice: windows
+    still hold and in a drafted row its descendants.  (1500 slots: windows
     shared by workgroups.)"""
-    say(f"tree {bad} kv={name} B={B}")
+    say(f"tree {bad} kv={name} B={B} C={C}")
     rng = np.random.default_rng(8)
-    C, T = 150, 20
-    pos0 = np.full(B, 400, np.int32)
-    pos0[0] = 260
+    T = 20
+    pos0 = np.full(B, C + 250, np.int32)
+    pos0[0] = C + 110
     n = np.full(B, T - 2, np.int32)
     qkv = rng.standard_normal((B, T, QKV), dtype=np.float32)
     parent = np.repeat(random_parents(rng, 1, T, 4), B, 0)
