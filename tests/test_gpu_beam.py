@@ -69,7 +69,7 @@ def test_beam_select(ctx, V, W, n):
         _check(got, logits, scores, n, done, end, seen, pen)
 
 
-@pytest.mark.parametrize("V", [100, 5000])
+@pytest.mark.parametrize("V", [100, 2000, 5000])
 def test_beam_ties(ctx, V):
     """Equal logits: the lower id; equal beams: the lower beam, whatever the
     place of a row in memory."""
@@ -82,7 +82,7 @@ def test_beam_ties(ctx, V):
     assert (parent[1] == 0).all() and np.array_equal(token[1], np.arange(12))
 
 
-@pytest.mark.parametrize("V", [70, 1024, 9000])
+@pytest.mark.parametrize("V", [70, 1024, 2000, 9000])
 def test_beam_first_step_and_not_finite(ctx, V):
     """Beams of score -inf or NaN do not go on; NaN and -inf logits are not
     chosen, a row of nothing else gives nothing; +inf logits share the whole."""
@@ -110,7 +110,7 @@ def test_beam_first_step_and_not_finite(ctx, V):
     assert list(got[2][1][:2]) == [0, 3] or set(got[2][1][:3]) == {0, 3, V - 1}
 
 
-@pytest.mark.parametrize("V,W", [(1024, 8), (7001, 5)])
+@pytest.mark.parametrize("V,W", [(1024, 8), (2001, 8), (7001, 5)])
 def test_beam_device_form(ctx, V, W):
     """bf16 logits (many ties) in rows at odd offsets, another stream, a
     workspace of any content, optional outputs left out."""
@@ -142,7 +142,7 @@ def test_beam_device_form(ctx, V, W):
         ctx.set_stream(None)
 
 
-@pytest.mark.parametrize("V", [1024, 9001])
+@pytest.mark.parametrize("V", [1024, 2001, 9001])
 def test_beam_graph_replays(ctx, V):
     """Captured and replayed with eager work between, every replay as the eager call."""
     import torch
